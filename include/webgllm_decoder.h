@@ -145,6 +145,25 @@ int wg_spec_accept(wg_ctx *ctx, const int32_t *drafts, const int32_t *picks, int
                    int32_t *pos_draft, int32_t *next_target, int32_t *next_draft, int32_t *out, int out_cap,
                    int32_t *out_len, int32_t *accepted);
 
+/* Sampled speculative decoding: verification of k drafted tokens per sequence
+ * against the target's probabilities, with given random numbers (the
+ * reference samples on the host, src/sampler.ts, and drafts greedily).
+ * target fp32 [k+1][batch][V] = the target's logits after the last kept token
+ * and after d_1..d_k, draft fp32 [k][batch][V] the logits the draft drew d_j
+ * from, drafts [batch][k], u fp32 [batch][k+1] in [0, 1). With p_j, q_j the
+ * softmax of row j over `temperature`: d_j is kept iff u_j q_j(d_j) <
+ * p_j(d_j); at the first that is not, the token is drawn from
+ * max(p_j - q_j, 0) by u_k (the first index whose running sum exceeds u_k
+ * times the total), and if all are kept from p_k. picks [k+1][batch] receives
+ * the kept tokens, the drawn one, then -1: wg_spec_accept with these picks
+ * keeps exactly that (the drawn token is never the rejected one). k = 0
+ * (draft and drafts NULL) is plain sampling. -inf logits (filtered tokens)
+ * have probability 0. The decisions are those of 64-bit arithmetic. A row
+ * with NaN, +inf or nothing but -inf yields some valid token and is reported
+ * by wg_sync. k <= 32, V <= 2^21, temperature in [1e-4, 1e4]. */
+int wg_spec_sample(wg_ctx *ctx, const float *target, const float *draft, const int32_t *drafts, int batch, int k,
+                   int V, double temperature, const float *u, int32_t *picks);
+
 /* counters[0..n) += delta on the device (advances the positions of a
  * replayed decode step). */
 int wg_add_i32(wg_ctx *ctx, int32_t *counters, int n, int delta);

@@ -35,6 +35,14 @@ class wg_prologue(ctypes.Structure):
                 ("weight", ctypes.c_void_p), ("eps", ctypes.c_float), ("resid_out", ctypes.c_void_p),
                 ("stats", ctypes.c_void_p)]
 
+
+class wg_paged_kv(ctypes.Structure):
+    """include/webgllm_paged.h wg_paged_kv."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("table", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("num_pages", ctypes.c_int), ("page_size", ctypes.c_int), ("max_pages", ctypes.c_int),
+                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
@@ -88,6 +96,11 @@ SIGNATURES = {
     "wg_argmax": (_I, [_P, _P, _I, _I, _P]),
     "wg_add_i32": (_I, [_P, _P, _I, _I]),
     "wg_spec_accept": (_I, [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P]),
+    "wg_spec_sample": (_I, [_P, _P, _P, _P, _I, _I, _I, ctypes.c_double, _P, _P]),
+    # include/webgllm_paged.h
+    "wg_paged_rope_kv": (_I, [_P, _P, _I, _I, _P, _I, _I, _I, _P, ctypes.c_double, _P, _P, ctypes.c_float, _P, _P]),
+    "wg_paged_attention": (_I, [_P, _P, _I, _I, _P, _I, _I, _I, _P, _P, _I, _I, _P, _P, _SZ]),
+    "wg_paged_attention_workspace": (_I, [_P, _I, ctypes.POINTER(_SZ)]),
     # include/webgllm_comm.h
     "wg_ipc_alloc": (_I, [_P, _SZ, _PP, _P]),
     "wg_ipc_free": (_I, [_P, _P]),

@@ -255,6 +255,27 @@ int wg_spec_accept(wg_ctx *ctx, const int32_t *drafts, const int32_t *picks, int
                 "wg_spec_accept");
 }
 
+int wg_spec_sample(wg_ctx *ctx, const float *target, const float *draft, const int32_t *drafts, int batch, int k,
+                   int V, double temperature, const float *u, int32_t *picks) {
+  WG_BEGIN(ctx);
+  if (batch < 0 || k < 0 || k > wg::kSampleMaxDrafts || V < 1 || V > wg::kSampleMaxVocab)
+    return dfail(ctx, WG_INVALID_SHAPE, "wg_spec_sample: batch %d, k %d (<= %d), V %d (<= %d)", batch, k,
+                 wg::kSampleMaxDrafts, V, wg::kSampleMaxVocab);
+  if (batch > (1 << 24)) return dfail(ctx, WG_UNSUPPORTED, "wg_spec_sample: batch %d", batch);
+  if (!(temperature >= 1e-4 && temperature <= 1e4))
+    return dfail(ctx, WG_INVALID_ARGUMENT, "wg_spec_sample: temperature %g outside [1e-4, 1e4]", temperature);
+  if (!batch) return WG_OK;
+  if (!target || !u || !picks || (k && (!draft || !drafts)))
+    return dfail(ctx, WG_INVALID_ARGUMENT, "wg_spec_sample: null");
+  for (const void *p : {(const void *)target, (const void *)draft, (const void *)drafts, (const void *)u,
+                        (const void *)picks})
+    if ((uintptr_t)p & 3u) return dfail(ctx, WG_INVALID_ARGUMENT, "wg_spec_sample: misaligned tensor");
+  return finish(ctx,
+                wg::launch_spec_sample(target, draft, drafts, batch, k, V, temperature, u, picks, ctx->d_flags,
+                                       ctx->stream, ctx->pdl),
+                "wg_spec_sample");
+}
+
 int wg_add_i32(wg_ctx *ctx, int32_t *counters, int n, int delta) {
   WG_BEGIN(ctx);
   if (n < 0) return dfail(ctx, WG_INVALID_SHAPE, "wg_add_i32: n %d", n);

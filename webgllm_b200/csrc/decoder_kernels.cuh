@@ -65,5 +65,10 @@ cudaError_t launch_add_i32(int32_t *p, int n, int delta, cudaStream_t s, bool pd
 cudaError_t launch_spec_accept(const int32_t *drafts, const int32_t *picks, int batch, int k, int32_t *pos_t,
                                int32_t *pos_d, int32_t *next_t, int32_t *next_d, int32_t *out, int out_cap,
                                int32_t *out_len, int32_t *accepted, cudaStream_t s, bool pdl);
+// spec_sample.cu
+constexpr int kSampleMaxDrafts = 32, kSampleMaxVocab = 1 << 21;
+cudaError_t launch_spec_sample(const float *target, const float *draft, const int32_t *drafts, int batch, int k, int V,
+                               double temperature, const float *u, int32_t *picks, unsigned *flags, cudaStream_t s,
+                               bool pdl);
 
 }  // namespace wg

@@ -31,6 +31,7 @@ import torch
 
 from . import _lib
 from .model import DecoderConfig, DecoderModel
+from .q4 import context
 
 P = ctypes.c_void_p
 
@@ -38,6 +39,43 @@ P = ctypes.c_void_p
 def draft_config(target: DecoderConfig) -> DecoderConfig:
     """Config 2's layout with the target's vocabulary."""
     return DecoderConfig("draft-1.1b", 22, 2048, 32, 4, 64, 5632, target.vocab, 1e-5, 1e4)
+
+
+def spec_sample(target: torch.Tensor, draft: torch.Tensor | None, drafts: torch.Tensor | None, u: torch.Tensor, *,
+                temperature: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """wg_spec_sample: verifies drafts int32 [batch][k] by the logits target
+    float32 [k + 1][batch][V] and draft float32 [k][batch][V] with the random
+    numbers u float32 [batch][k + 1]. Returns picks int32 [k + 1][batch]: the
+    kept tokens, then the drawn one, then -1 (what wg_spec_accept takes).
+    draft and drafts None (k = 0): one token per sequence drawn from target
+    [1][batch][V] (or [batch][V])."""
+    if target.dim() == 2 and draft is None:
+        target = target.unsqueeze(0)
+    device = target.device
+    if target.dim() != 3 or not target.is_cuda:
+        raise _lib.ShapeError(_lib.WG_INVALID_SHAPE, f"target {tuple(target.shape)} must be CUDA logits [k + 1][batch][V]")
+    k, batch, V = target.shape[0] - 1, target.shape[1], target.shape[2]
+    if (draft is None) != (k == 0) or (drafts is None) != (k == 0):
+        raise _lib.ShapeError(_lib.WG_INVALID_SHAPE, f"{k} drafted tokens a sequence need their draft logits and drafts")
+    want = [(target, torch.float32, target.shape, "target"), (u, torch.float32, (batch, k + 1), "u")]
+    if k:
+        want += [(draft, torch.float32, (k, batch, V), "draft"), (drafts, torch.int32, (batch, k), "drafts")]
+    if out is None:
+        out = torch.empty((k + 1, batch), dtype=torch.int32, device=device)
+    else:
+        want.append((out, torch.int32, (k + 1, batch), "out"))
+    for t, dt, shape, what in want:
+        if t.shape != shape:
+            raise _lib.ShapeError(_lib.WG_INVALID_SHAPE, f"{what} {tuple(t.shape)} must be {tuple(shape)}")
+        if t.dtype != dt or t.device != device or not t.is_contiguous():
+            raise _lib.GpuError(_lib.WG_INVALID_ARGUMENT, f"{what} must be contiguous {dt} on {device}")
+    ctx = context(device.index)
+    ctx.use_torch_stream()
+    with torch.cuda.device(device):
+        ctx._check(_lib.lib().wg_spec_sample(ctx.handle, target.data_ptr(), draft.data_ptr() if k else None,
+                                             drafts.data_ptr() if k else None, batch, k, V, temperature, u.data_ptr(),
+                                             out.data_ptr()))
+    return out
 
 
 class SpeculativeDecoder:
