@@ -1,52 +1,13 @@
 // The paged key-value cache (webgllm_paged.h): the append of new rows (qk-norm
 // and RoPE on the way) and attention over the pages.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <cmath>
-#include <type_traits>
 
 #include "common.cuh"
-#include "device_utils.cuh"
-#include "paged.cuh"
-#include "tma.cuh"
+#include "paged_device.cuh"
 
 namespace wg {
 
 namespace {
-
-// ---- 16-bit types ----------------------------------------------------------
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t u);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
-  return __half22float2(*reinterpret_cast<const __half2 *>(&u));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u));
-}
-
-// Whether a packed pair holds an infinity or NaN (exponent bits all ones).
-template <typename T>
-__device__ __forceinline__ bool nonfinite2(uint32_t u) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-  return (u & e) == e || (u >> 16 & e) == e;
-}
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -74,17 +35,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t r[4]) {
 }
 
 // ---- rows and sequences ----------------------------------------------------
-
-// Rows of sequence b: [r0, r0 + n), clamped to the buffers.
-__device__ __forceinline__ void seq_rows(const PagedRows &a, int b, int &r0, int &n) {
-  if (a.row_start) {
-    r0 = min(max(a.row_start[b], 0), a.rows);
-    n = max(min(a.row_start[b + 1], a.rows) - r0, 0);
-  } else {
-    n = a.rows / a.batch;
-    r0 = b * n;
-  }
-}
 
 // The sequence of row r (by the whole warp), or -1 if it belongs to none:
 // the last b with row_start[b] <= r, found 32 entries at a step.
@@ -266,15 +216,11 @@ struct SplitArgs {
   unsigned *flags;
 };
 
-// One sequence's share of the work.
-struct SeqWork {
-  int r0, n;    // rows
-  int p;        // position of its first row
-  int mt;       // row tiles
-  int hi;       // keys [0, hi) are seen by some row, but for [se, ws)
-  int ws, se;   // window start of the first row, end of the sinks
-  int a, c;     // key tiles: [0, a) and [c, c + nt - a)
-  int nt;
+// One sequence's share of the work: row tiles (per KV head) times key tiles.
+struct SeqWork : KeySpan {
+  int r0, n;  // rows
+  int p;      // position of its first row
+  int mt;     // row tiles
 };
 
 __device__ __forceinline__ SeqWork seq_work(const SplitArgs &A, int b, int rows_per_tile) {
@@ -282,15 +228,7 @@ __device__ __forceinline__ SeqWork seq_work(const SplitArgs &A, int b, int rows_
   seq_rows(A.pr, b, w.r0, w.n);
   w.p = A.pr.pos[b];
   w.mt = (int)(((long long)w.n * A.G + rows_per_tile - 1) / rows_per_tile);
-  const long long cap = (long long)A.pt.max_pages * A.pt.page_size;
-  const long long last = (long long)w.p + w.n;
-  w.hi = (int)max(0LL, min(last, cap));
-  w.ws = A.window > 0 ? (int)min((long long)w.hi, max(0LL, (long long)w.p - A.window + 1)) : 0;
-  w.se = min(A.sinks, w.ws);
-  w.a = (w.se + kKeys - 1) / kKeys;
-  w.c = max(w.ws / kKeys, w.a);
-  w.nt = w.a + max(0, (w.hi + kKeys - 1) / kKeys - w.c);
-  if (w.nt == 0) w.nt = 1;  // rows that see nothing still get their zeros
+  static_cast<KeySpan &>(w) = key_span(w.p, w.n, A.window, A.sinks, A.pt, kKeys);
   return w;
 }
 
@@ -443,11 +381,7 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
           uint8_t *dst = smem + (size_t)stage * S::kStageBytes + is_v * S::kTileBytes + blk * kBlkBytes +
                          box * box_bytes;
           const CUtensorMap *tm = is_v ? &tm_v : &tm_k;
-          asm volatile(
-              "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, "
-              "%6}], [%2];" ::"r"(smem_u32(dst)),
-              "l"(tm), "r"(smem_u32(&full[stage])), "r"(blk * 64), "r"(key % A.pt.page_size), "r"(hk), "r"(page)
-              : "memory");
+          tma_load_4d(dst, tm, blk * 64, key % A.pt.page_size, hk, page, &full[stage]);
         }
         page = page_next;
         key = key_next;
@@ -569,8 +503,7 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                   const int key = key0 + nt * 8 + 2 * t4 + (e & 1), p = rp[mt][e >> 1];
-                  const bool see = key <= p && key < w.hi && (A.window == 0 || key > p - A.window || key < A.sinks);
-                  if (!see) s[mt][nt][e] = -INFINITY;
+                  if (key >= w.hi || !sees_key(p, key, A.window, A.sinks)) s[mt][nt][e] = -INFINITY;
                 }
           }
           // online softmax; the probabilities as hi + lo halves
@@ -584,7 +517,7 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
               const float mn = fmaxf(mx[mt][e], m * kLog2e);
-              f[e] = mn == -INFINITY ? 1.0f : exp2f(mx[mt][e] - mn);
+              f[e] = mn == -INFINITY ? 1.0f : ex2(mx[mt][e] - mn);
               const float sub = mn == -INFINITY ? 0.0f : mn;
               mx[mt][e] = mn;
               float sum = 0.0f;
@@ -592,7 +525,7 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
               for (int nt = 0; nt < 2; nt++)
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                  const float v = exp2f(s[mt][nt][2 * e + c] * kLog2e - sub);
+                  const float v = ex2(s[mt][nt][2 * e + c] * kLog2e - sub);
                   s[mt][nt][2 * e + c] = v;
                   sum += v;
                 }
@@ -645,7 +578,7 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
                   const float hi = kr < 8 ? s[mt][0][2 * e + 1] : s[mt][1][2 * e + 1];
                   pv[e] = __shfl_sync(0xffffffffu, kr & 1 ? hi : lo, src);
                   const int p = rp[mt][e];
-                  see[e] = key <= p && key < w.hi && (A.window == 0 || key > p - A.window || key < A.sinks);
+                  see[e] = key < w.hi && sees_key(p, key, A.window, A.sinks);
                 }
 #pragma unroll
                 for (int d = 0; d < Dh / 8; d++) {
@@ -695,7 +628,7 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
           float m = -INFINITY;
 #pragma unroll
           for (int i = 0; i < kSplitWarps; i++) m = fmaxf(m, sm_m[i * S::kRows + row]);
-          const float f = m == -INFINITY ? 0.0f : exp2f(mx[mt][e] - m);
+          const float f = m == -INFINITY ? 0.0f : ex2(mx[mt][e] - m);
 #pragma unroll
           for (int d = 0; d < Dh / 8; d++) {
             o[mt][d][2 * e] *= f;
@@ -741,7 +674,7 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
         for (int k = 0; k < kSplitWarps; k++) mm = fmaxf(mm, sm_m[k * S::kRows + row]);
 #pragma unroll
         for (int k = 0; k < kSplitWarps; k++)
-          l += mm == -INFINITY ? 0.0f : sm_l[k * S::kRows + row] * exp2f(sm_m[k * S::kRows + row] - mm);
+          l += mm == -INFINITY ? 0.0f : sm_l[k * S::kRows + row] * ex2(sm_m[k * S::kRows + row] - mm);
         const float4 x = *reinterpret_cast<const float4 *>(red + row * Dh + d);
         const float4 y = *reinterpret_cast<const float4 *>(red + (S::kRows + row) * Dh + d);
         float4 v = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
@@ -817,7 +750,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const int *rec
 #pragma unroll 4
   for (int j = grp; j < np; j += kGroups) {
     const float *p = part(j);
-    const float f = mm == -INFINITY ? 0.0f : exp2f(p[row] - mm);
+    const float f = mm == -INFINITY ? 0.0f : ex2(p[row] - mm);
     const float4 v = *reinterpret_cast<const float4 *>(p + 2 * unit_rows + (size_t)row * Dh + lane * 4);
     a.x += v.x * f;
     a.y += v.y * f;
@@ -846,24 +779,6 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const int *rec
   }
 }
 
-template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s, bool pdl,
-                   const Args &...args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  if (pdl) {
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-  }
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
-}
-
 int64_t stride_or(int64_t s, int64_t dense) { return s ? s : dense; }
 
 template <typename T, int Dh>
@@ -883,24 +798,9 @@ cudaError_t rope_t(const float *qkv, const PagedRows &pr, int H, int Hkv, const 
                 ps = stride_or(kv.page_stride, (int64_t)Hkv * kv.page_size * Dh);
   const int threads = warps <= num_sms * 4 ? 64 : 256;
   const unsigned blocks = (unsigned)((warps * 32 + threads - 1) / threads);
-  return launch(paged_rope_kernel<T, Dh>, dim3(blocks), threads, 0, s, pdl, qkv, pr, H, Hkv, turns, q_norm, k_norm, eps,
+  return launch_pdl(paged_rope_kernel<T, Dh>, dim3(blocks), threads, 0, s, pdl, qkv, pr, H, Hkv, turns, q_norm, k_norm, eps,
                 reinterpret_cast<T *>(q_out), reinterpret_cast<T *>(kv.k), reinterpret_cast<T *>(kv.v), ps, hs, rs, pt,
                 hpw, wpr, flags);
-}
-
-// The pages as a tensor of (dim, row in page, head, page).
-bool page_map(CUtensorMap *m, void *base, const wg_paged_kv &kv, int Hkv, int Dh, int box_rows) {
-  EncodeTiled enc = encode_fn();
-  if (!enc) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)Dh, (cuuint64_t)kv.page_size, (cuuint64_t)Hkv, (cuuint64_t)kv.num_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)stride_or(kv.row_stride, Dh) * 2,
-                                 (cuuint64_t)stride_or(kv.head_stride, (int64_t)kv.page_size * Dh) * 2,
-                                 (cuuint64_t)stride_or(kv.page_stride, (int64_t)Hkv * kv.page_size * Dh) * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-  const cuuint32_t one[4] = {1, 1, 1, 1};
-  return enc(m, kv.dtype == WG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims,
-             strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 constexpr int split_ctas_per_sm(int Dh, int MT) { return MT == 1 && Dh <= 128 ? 2 : 1; }
@@ -924,12 +824,12 @@ cudaError_t split_t(SplitArgs A, const wg_paged_kv &kv, void *workspace, int num
   const int P = num_sms * occ;
   A.rec = reinterpret_cast<int *>(workspace);
   A.part = reinterpret_cast<float *>(A.rec + (size_t)P * 8);
-  e = launch(kern, dim3((unsigned)P), kSplitThreads, smem, s, pdl, tk, tv, A);
+  e = launch_pdl(kern, dim3((unsigned)P), kSplitThreads, smem, s, pdl, tk, tv, A);
   if (e != cudaSuccess) return e;
   // rows of a unit that can exist: none past the longest sequence's
   const long long most = A.pr.row_start ? A.pr.rows : A.pr.rows / A.pr.batch;
   const unsigned rows = (unsigned)(most * A.G < S::kRows ? most * A.G : S::kRows);
-  return launch(paged_join_kernel<T, Dh>, dim3((unsigned)P, rows), kJoinThreads, 0, s, pdl, A.rec, A.part, S::kRows,
+  return launch_pdl(paged_join_kernel<T, Dh>, dim3((unsigned)P, rows), kJoinThreads, 0, s, pdl, A.rec, A.part, S::kRows,
                 A.H, A.G, reinterpret_cast<T *>(A.out));
 }
 
@@ -988,6 +888,8 @@ size_t paged_attention_workspace(int Dh, int num_sms) {
 cudaError_t launch_paged_attention(const void *q, const PagedRows &rows, int H, int Hkv, int Dh,
                                    const wg_paged_kv &kv, int window, int sinks, void *out, void *workspace,
                                    unsigned *flags, int num_sms, cudaStream_t s, bool pdl) {
+  if (paged_prompt_supported(rows, H, Hkv, num_sms))
+    return launch_paged_prompt(q, rows, H, Hkv, Dh, kv, window, sinks, out, flags, num_sms, s, pdl);
   SplitArgs A{};
   A.pr = rows;
   A.pt = PagedTable{kv.table, kv.max_pages, kv.num_pages, kv.page_size};

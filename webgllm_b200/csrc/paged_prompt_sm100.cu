@@ -1,0 +1,639 @@
+// Attention of many rows over the paged cache (prompt chunks) on the Blackwell
+// tensor cores: the same operator as paged.cu's split kernel, for shapes that
+// are bound by the products instead of the reads.
+//
+// A unit is (sequence, KV head, NT tiles of 128 query rows); a tile's rows are
+// RP = 128 / G consecutive rows of the sequence times the G query heads of the
+// KV head, so that one K / V tile serves the whole group and a tile spans few
+// positions (little of it is cut by the causal border). Persistent CTAs, one an
+// SM, take units round robin, longest first. Per CTA:
+//   warps 0 .. 4 NT - 1  softmax: a thread owns a row. tcgen05.ld of the row's
+//                scores, mask, maximum, exp2, P as 16-bit pairs back into the
+//                scores' tensor-memory columns (the A operand of P V), the row
+//                sum in a register; at the end O from tensor memory to `out`.
+//                The reference maximum follows the true one only when that
+//                has grown by 2^8 (P stays below 2^8, well inside fp16): O is
+//                then rescaled in tensor memory, which almost never happens
+//                after the first tiles;
+//   one warp     MMA: one thread issues S_t = Q_t K^T (both operands in shared
+//                memory) and O_t += P_t V (P from tensor memory, V as it lies,
+//                [key][dim], the MN-major form). The two tiles alternate:
+//                while one's softmax runs, the other's products do;
+//   one warp     loads: Q by one 3-D TMA box a tile and 64 dims, K and V by the
+//                boxes of pages into a ring of stages;
+//   one warp     cleans V tiles that not every row sees in full: rows that no
+//                row sees become zeros (their P is 0, but 0 times what a page
+//                holds there need not be), and infinities or NaN in the others
+//                are set aside (P = 0 must not meet them) and added at the end
+//                for the rows that do see them.
+// Every MMA is issued by one thread, so they execute in order: S_t(j + 1) may
+// overwrite P_t(j) after P V(j) was issued, and the commit that reports
+// S_t(j) reports P_t(j - 1) V too.
+// Waits are bounded, and tensor memory is freed on every path.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "paged_device.cuh"
+
+namespace wg {
+
+namespace {
+
+// Entries by key tile (not by stage: a stage carries K of one round and V of
+// another): which page boxes of the tile were loaded; whether its V is clean.
+constexpr int kHeldRing = 8;
+constexpr int kOddRing = 8, kOddMax = 14;
+
+template <int Dh_>
+struct PromptCfg {
+  static constexpr int Dh = Dh_;
+  static constexpr int NT = Dh == 256 ? 1 : 2;   // query tiles of a CTA
+  static constexpr int KT = Dh == 256 ? 64 : 128;  // keys of a tile
+  static constexpr int kQBytes = 128 * Dh * 2;     // one query tile
+  static constexpr int kStageBytes = KT * Dh * 2;  // K or V of a key tile
+  static constexpr int kStages = (224 * 1024 - NT * kQBytes) / kStageBytes > 8 ? 8
+                                 : (224 * 1024 - NT * kQBytes) / kStageBytes;
+  static constexpr int kThreads = (4 * NT + 3) * 32;
+  static constexpr int kSmem = 1024 + NT * kQBytes + kStages * kStageBytes;
+  static constexpr int kOCol = 256;  // tensor memory: scores at [0, 256), O after them
+  static constexpr int kSCol = NT == 2 ? 128 : 64;  // columns between the two score buffers
+};
+
+struct PromptArgs {
+  PagedRows pr;
+  PagedTable pt;
+  void *out;
+  const void *v;  // for values set aside
+  int64_t page_stride, head_stride, row_stride;
+  int H, Hkv, G, RP;
+  int window, sinks;
+  int box_rows;
+  unsigned *flags;
+};
+
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tc_commit_to(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+// D (+)= A B with A and B in shared memory, or A in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// Shared-memory descriptor, 128-byte swizzle: 8-row groups 1024 bytes apart
+// (SBO), and for the MN-major form `lbo` bytes between 64-element blocks.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// kind::f16, M = 128: A and B of type T (K-major, or B MN-major), fp32 sums.
+template <typename T>
+__host__ __device__ constexpr uint32_t instr_desc(int N, bool b_mn) {
+  return (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | (b_mn ? 1u << 16 : 0u) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float *v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+struct Unit : KeySpan {
+  int b, hk, r0, n, p;
+  int i0;  // first row of its NT tiles
+};
+
+// The units in order: sequence, then the rows from the last to the first, then
+// the KV head. Each role of a CTA walks the same ones.
+struct UnitWalk {
+  int b = 0;
+  long long base = 0;
+  __device__ bool get(const PromptArgs &A, long long item, int rows_per_unit, int KT, Unit &u) {
+    for (; b < A.pr.batch; b++) {
+      seq_rows(A.pr, b, u.r0, u.n);
+      const int chunks = (u.n + rows_per_unit - 1) / rows_per_unit;
+      const long long cnt = (long long)chunks * A.Hkv;
+      if (item < base + cnt) {
+        const long long local = item - base;
+        u.b = b;
+        u.p = A.pr.pos[b];
+        u.i0 = (chunks - 1 - (int)(local / A.Hkv)) * rows_per_unit;
+        u.hk = (int)(local % A.Hkv);
+        static_cast<KeySpan &>(u) =
+            key_span((long long)u.p + u.i0, min(u.n - u.i0, rows_per_unit), A.window, A.sinks, A.pt, KT);
+        return true;
+      }
+      base += cnt;
+    }
+    return false;
+  }
+};
+
+template <typename T, int Dh>
+__global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
+    paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, const PromptArgs A) {
+  using C = PromptCfg<Dh>;
+  constexpr int NT = C::NT, KT = C::KT, S = C::kStages;
+  constexpr int kBlk = Dh / 64, kBlkBytes = KT * 128;
+  constexpr float kLog2e = 1.4426950408889634f;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t *ring = smem + NT * C::kQBytes;
+  __shared__ uint64_t q_full, q_empty, kv_full[S], kv_empty[S], v_ready[kHeldRing], s_full[2], p_full[2], o_full[2], o_empty[2],
+      pv_done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int held[kHeldRing];
+  __shared__ int odd[kOddRing][kOddMax + 2];  // [0]: how many, then the tiles
+  __shared__ int aborted;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int w_mma = 4 * NT, w_load = 4 * NT + 1;
+  const int rows_per_unit = NT * A.RP;
+  constexpr int kAll = (1 << (KT / 16)) - 1;
+
+  if (tid == 0) {
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1);
+    for (int i = 0; i < S; i++) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < kHeldRing; i++) mbar_init(&v_ready[i], 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 4);
+    }
+    mbar_init(&pv_done, 1);
+    fence_mbar_init();
+    aborted = 0;
+  }
+  if (warp == w_mma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == w_load && lane == 0) {
+    prefetch_tensormap(&tm_q);
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+  }
+  pdl_trigger();
+  pdl_wait();
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_slot;
+
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if (*(volatile int *)&aborted) return;
+    if (!mbar_wait_bounded(bar, parity, A.flags)) *(volatile int *)&aborted = 1;
+  };
+  // whether every row of the unit sees every key of tile t
+  auto open_tile = [&](const Unit &u, int key0) {
+    const long long first = (long long)u.p + u.i0, last = (long long)u.p + min(u.n, u.i0 + rows_per_unit) - 1;
+    return key0 + KT - 1 <= first &&
+           (A.window == 0 || key0 + KT - 1 < A.sinks || (long long)key0 > last - A.window);
+  };
+  auto tile_key = [&](const Unit &u, int t) { return (t < u.a ? t : t - u.a + u.c) * KT; };
+
+  UnitWalk walk;
+  Unit u;
+  if (warp == w_load) {
+    // ---- loads ----
+    const int nb = KT / A.box_rows, nops = nb * kBlk;
+    const int box = lane % nb, blk = lane / nb;
+    const uint32_t box_bytes = (uint32_t)A.box_rows * 128;
+    const int groups = A.box_rows / 16, gmask = (1 << groups) - 1;
+    int stage = 0, phase = 0, nu = 0, nt = 0;
+    for (long long item = blockIdx.x; walk.get(A, item, rows_per_unit, KT, u); item += gridDim.x, nu++) {
+      wait(&q_empty, (nu & 1) ^ 1);
+      if (lane == 0) {
+        mbar_expect_tx(&q_full, (uint32_t)(NT * kBlk * A.G * A.RP * 128));
+        for (int t = 0; t < NT; t++)
+          for (int i = 0; i < kBlk; i++)
+            tma_load_3d(smem + t * C::kQBytes + i * 16384, &tm_q, i * 64, u.hk * A.G, u.r0 + u.i0 + t * A.RP, &q_full);
+      }
+      const int32_t *row = A.pt.table + (size_t)u.b * A.pt.max_pages;
+      auto entry = [&](int t, int &key, bool &seen) {
+        key = tile_key(u, t) + box * A.box_rows;
+        seen = lane < nops && key < u.hi && (key < u.se || key + A.box_rows > u.ws);
+        return seen ? row[key / A.pt.page_size] : -1;
+      };
+      int key, key_next = 0;
+      bool seen, seen_next = false;
+      int page = entry(0, key, seen), page_next = -1;
+      for (int t = 0; t < u.nt; t++, nt++) {
+        if (t + 1 < u.nt) page_next = entry(t + 1, key_next, seen_next);
+        const bool ok = seen && page >= 0 && page < A.pt.num_pages;
+        if (seen && !ok) raise_flag(A.flags, kFlagBadArgument);
+        const unsigned loaded = __ballot_sync(0xffffffffu, ok && lane < nb);
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {  // K, then V
+          wait(&kv_empty[stage], phase ^ 1);
+          if (lane == 0) {
+            if (kv == 0) {
+              int m = 0;
+              for (int i = 0; i < nb; i++)
+                if (loaded >> i & 1) m |= gmask << (i * groups);
+              held[nt % kHeldRing] = m;
+            }
+            mbar_expect_tx(&kv_full[stage], (uint32_t)__popc(loaded) * box_bytes * kBlk);
+          }
+          __syncwarp();
+          if (ok)
+            tma_load_4d(ring + (size_t)stage * C::kStageBytes + blk * kBlkBytes + box * box_bytes, kv ? &tm_v : &tm_k,
+                        blk * 64, key % A.pt.page_size, u.hk, page, &kv_full[stage]);
+          if (++stage == S) stage = 0, phase ^= 1;
+        }
+        page = page_next;
+        key = key_next;
+        seen = seen_next;
+      }
+    }
+    // after a wait that ran out, no copy may still be on its way when the CTA exits
+    __syncwarp();
+    if (*(volatile int *)&aborted && lane == 0) {
+      for (int i = 0; i < S; i++) {
+        mbar_wait_bounded(&kv_full[stage], phase ^ 1, A.flags);
+        if (++stage == S) stage = 0, phase ^= 1;
+      }
+      if (nu) mbar_wait_bounded(&q_full, (nu - 1) & 1, A.flags);
+    }
+  } else if (warp == w_mma) {
+    // ---- products ----
+    if (lane == 0) {
+      constexpr uint32_t qk_desc = instr_desc<T>(KT, false), pv_desc = instr_desc<T>(Dh, true);
+      int stage = 0, phase = 0, nu = 0, np = 0;
+      auto step = [&](int &s, int &ph) {
+        if (++s == S) s = 0, ph ^= 1;
+      };
+      // S_x = Q_t K^T
+      auto qk = [&](int t, int x, int st) {
+        const uint32_t q = smem_u32(smem) + t * C::kQBytes, k = smem_u32(ring) + st * C::kStageBytes;
+#pragma unroll
+        for (int kk = 0; kk < Dh / 16; kk++)
+          mma_ss(tmem + x * C::kSCol, smem_desc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16),
+                 smem_desc(k + (kk >> 2) * kBlkBytes + (kk & 3) * 32, 16), qk_desc, kk > 0);
+      };
+      auto pv = [&](int t, int x, int st, bool first) {
+        const uint32_t v = smem_u32(ring) + st * C::kStageBytes;
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; kk++)
+          mma_ts(tmem + C::kOCol + t * Dh, tmem + x * C::kSCol + kk * 8, smem_desc(v + kk * 2048, kBlkBytes), pv_desc,
+                 !(first && kk == 0));
+      };
+      for (long long item = blockIdx.x; walk.get(A, item, rows_per_unit, KT, u); item += gridDim.x, nu++) {
+        wait(&q_full, nu & 1);
+        wait(&kv_full[stage], phase);  // K of tile 0
+        tc_after();
+        if constexpr (NT == 2) {
+          for (int t = 0; t < 2; t++) {
+            qk(t, t, stage);
+            tc_commit_to(&s_full[t]);
+          }
+          tc_commit_to(&kv_empty[stage]);
+          step(stage, phase);
+          for (int j = 0; j < u.nt; j++, np++) {
+            const int vs = stage;
+            step(stage, phase);
+            const bool more = j + 1 < u.nt;
+            if (!more) tc_commit_to(&q_empty);
+            wait(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
+            for (int t = 0; t < 2; t++) {
+              wait(&p_full[t], np & 1);
+              if (j == 0) wait(&o_empty[t], (nu & 1) ^ 1);
+              tc_after();
+              pv(t, t, vs, j == 0);
+              if (t == 1) tc_commit_to(&kv_empty[vs]);
+              if (!more) tc_commit_to(&o_full[t]);
+              if (more) {
+                if (t == 0) {
+                  wait(&kv_full[stage], phase);
+                  tc_after();
+                }
+                qk(t, t, stage);
+                tc_commit_to(&s_full[t]);
+                if (t == 1) tc_commit_to(&kv_empty[stage]);
+              }
+            }
+            if (more) step(stage, phase);
+          }
+        } else {
+          // one tile of rows, two buffers of scores: S(j + 1) is made while S(j)
+          // is in softmax
+          qk(0, np & 1, stage);
+          tc_commit_to(&s_full[np & 1]);
+          tc_commit_to(&kv_empty[stage]);
+          step(stage, phase);
+          for (int j = 0; j < u.nt; j++, np++) {
+            const int vs = stage;
+            step(stage, phase);
+            if (j + 1 < u.nt) {
+              wait(&kv_full[stage], phase);
+              tc_after();
+              qk(0, (np + 1) & 1, stage);
+              tc_commit_to(&s_full[(np + 1) & 1]);
+              tc_commit_to(&kv_empty[stage]);
+              step(stage, phase);
+            } else {
+              tc_commit_to(&q_empty);
+            }
+            wait(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
+            wait(&p_full[np & 1], (np >> 1) & 1);
+            if (j == 0) wait(&o_empty[0], (nu & 1) ^ 1);
+            tc_after();
+            pv(0, np & 1, vs, j == 0);
+            tc_commit_to(&kv_empty[vs]);
+            tc_commit_to(&pv_done);
+            if (j + 1 == u.nt) tc_commit_to(&o_full[0]);
+          }
+        }
+      }
+    }
+  } else if (warp == w_load + 1) {
+    // ---- V tiles that some rows do not see in full ----
+    int stage = 0, phase = 0, nu = 0, nt = 0;
+    for (long long item = blockIdx.x; walk.get(A, item, rows_per_unit, KT, u); item += gridDim.x, nu++) {
+      int *list = odd[nu % kOddRing];
+      int nodd = 0;
+      for (int t = 0; t < u.nt; t++, nt++) {
+        if (++stage == S) stage = 0, phase ^= 1;  // past K
+        wait(&kv_full[stage], phase);
+        const int key0 = tile_key(u, t), m = held[nt % kHeldRing];
+        if (!open_tile(u, key0) || m != kAll) {
+          bool found = false;
+          uint8_t *v = ring + (size_t)stage * C::kStageBytes;
+          for (int i = lane; i < KT * (Dh / 8); i += 32) {
+            const int kr = i / (Dh / 8), ch = i - kr * (Dh / 8), key = key0 + kr;
+            uint4 *at =
+                reinterpret_cast<uint4 *>(v + (ch >> 3) * kBlkBytes + kr * 128 + (((ch & 7) ^ (kr & 7)) << 4));
+            if (key >= u.hi || (key >= u.se && key < u.ws) || !(m >> (kr >> 4) & 1)) {
+              *at = make_uint4(0, 0, 0, 0);
+            } else {
+              uint4 x = *at;
+              uint32_t w[4] = {x.x, x.y, x.z, x.w};
+              bool here = false;
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                constexpr uint32_t ex = kNonfinite<T>;
+                if ((w[e] & ex) == ex) w[e] &= 0xFFFF0000u, here = true;
+                if ((w[e] >> 16 & ex) == ex) w[e] &= 0xFFFFu, here = true;
+              }
+              if (here) *at = make_uint4(w[0], w[1], w[2], w[3]);
+              found |= here;
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          if (__any_sync(0xffffffffu, found) && nodd < kOddMax) {
+            if (lane == 0) list[1 + nodd] = t;
+            nodd++;
+          }
+        }
+        if (t + 1 == u.nt && lane == 0) list[0] = nodd;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ready[nt % kHeldRing]);
+        if (++stage == S) stage = 0, phase ^= 1;
+      }
+    }
+  } else {
+    // ---- softmax: one row a thread ----
+    const int t = warp >> 2, m = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t o_addr = tmem + lanes + C::kOCol + t * Dh;
+    const int i_in = m / A.G, g = m - i_in * A.G;
+    int nu = 0, np = 0;
+    for (long long item = blockIdx.x; walk.get(A, item, rows_per_unit, KT, u); item += gridDim.x, nu++) {
+      const int i = u.i0 + t * A.RP + i_in;
+      const bool valid = i_in < A.RP && i < u.n;
+      const int p = valid ? (int)max(-1LL, min((long long)u.p + i, 0x7ffffffeLL)) : -1;
+      float ref = -INFINITY, l = 0.0f;  // the reference maximum (log2 units) and the row sum over it
+      for (int j = 0; j < u.nt; j++, np++) {
+        const int x = NT == 2 ? t : np & 1;
+        const uint32_t s_addr = tmem + lanes + x * C::kSCol;
+        wait(&s_full[x], NT == 2 ? np & 1 : (np >> 1) & 1);
+        tc_after();
+        float s[KT];
+#pragma unroll
+        for (int c = 0; c < KT / 32; c++) tmem_ld32(s_addr + c * 32, s + c * 32);
+        tmem_wait_ld();
+        const int key0 = tile_key(u, j), hm = held[np % kHeldRing];
+        if (!open_tile(u, key0) || hm != kAll) {
+#pragma unroll
+          for (int c = 0; c < KT; c++) {
+            const int key = key0 + c;
+            if (!(hm >> (c >> 4) & 1) || key >= u.hi || !sees_key(p, key, A.window, A.sinks)) s[c] = -INFINITY;
+          }
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < KT; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
+        const bool grow = top > ref + 8.0f || (ref == -INFINITY && top > -INFINITY);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = grow ? (ref == -INFINITY ? 0.0f : ex2(ref - top)) : 1.0f;
+          if (grow) {
+            ref = top;
+            l *= f;
+          }
+          if (j > 0) {
+            // O holds the tiles before this one: with two row tiles the commit
+            // of these scores covers them, with one it does not
+            if constexpr (NT == 1) wait(&pv_done, (np - 1) & 1);
+            tc_after();
+#pragma unroll 1
+            for (int c = 0; c < Dh / 32; c++) {
+              float o[32];
+              tmem_ld32(o_addr + c * 32, o);
+              tmem_wait_ld();
+              uint32_t r[32];
+#pragma unroll
+              for (int e = 0; e < 32; e++) r[e] = __float_as_uint(o[e] * f);
+              tmem_st32(o_addr + c * 32, r);
+            }
+          }
+        }
+        const float sub = ref == -INFINITY ? 0.0f : ref;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < KT / 64; c++) {
+          uint32_t r[32];
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            const float a = ex2(fmaf(s[c * 64 + 2 * e], kLog2e, -sub));
+            const float b = ex2(fmaf(s[c * 64 + 2 * e + 1], kLog2e, -sub));
+            sum[e & 3] += a + b;
+            r[e] = pack2<T>(a, b);
+          }
+          tmem_st32(s_addr + c * 32, r);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+      }
+      // ---- the rows' results
+      wait(&o_full[t], nu & 1);
+      tc_after();
+      const int *list = odd[nu % kOddRing];
+      const int nodd = list[0];
+      const float inv = ref == -INFINITY ? 0.0f : 1.0f / l;
+      T *dst = reinterpret_cast<T *>(A.out) + ((size_t)(u.r0 + i) * A.H + u.hk * A.G + g) * Dh;
+#pragma unroll 1
+      for (int c = 0; c < Dh / 32; c++) {
+        float o[32];
+        tmem_ld32(o_addr + c * 32, o);
+        tmem_wait_ld();
+        if (nodd && valid) {
+          // infinities and NaN of V that this row does see
+          for (int k = 0; k < nodd; k++) {
+            const int key0 = tile_key(u, list[1 + k]);
+            for (int key = key0; key < key0 + KT; key++) {
+              if (key >= u.hi || !sees_key(p, key, A.window, A.sinks)) continue;
+              const int page = A.pt.table[(size_t)u.b * A.pt.max_pages + key / A.pt.page_size];
+              if (page < 0 || page >= A.pt.num_pages) continue;
+              const uint32_t *v = reinterpret_cast<const uint32_t *>(
+                  reinterpret_cast<const T *>(A.v) + page * A.page_stride + u.hk * A.head_stride +
+                  (key % A.pt.page_size) * A.row_stride + c * 32);
+#pragma unroll
+              for (int e = 0; e < 16; e++) {
+                const uint32_t w = v[e];
+                const float2 f = unpack2<T>(w);
+                if ((w & kNonfinite<T>) == kNonfinite<T>) o[2 * e] += f.x;
+                if ((w >> 16 & kNonfinite<T>) == kNonfinite<T>) o[2 * e + 1] += f.y;
+              }
+            }
+          }
+        }
+        if (valid) {
+          // a row that saw nothing: O may hold anything, its result is zeros
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            uint4 r = make_uint4(0, 0, 0, 0);
+            if (ref > -INFINITY || isnan(l)) {
+              r.x = pack2<T>(o[8 * e] * inv, o[8 * e + 1] * inv);
+              r.y = pack2<T>(o[8 * e + 2] * inv, o[8 * e + 3] * inv);
+              r.z = pack2<T>(o[8 * e + 4] * inv, o[8 * e + 5] * inv);
+              r.w = pack2<T>(o[8 * e + 6] * inv, o[8 * e + 7] * inv);
+            }
+            *reinterpret_cast<uint4 *>(dst + c * 32 + 8 * e) = r;
+          }
+        }
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_empty[t]);
+    }
+  }
+
+  tc_before();
+  __syncthreads();
+  if (warp == w_mma) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+template <typename T, int Dh>
+cudaError_t prompt_t(const void *q, PromptArgs A, const wg_paged_kv &kv, int num_sms, cudaStream_t s, bool pdl) {
+  using C = PromptCfg<Dh>;
+  auto kern = paged_prompt_kernel<T, Dh>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return e;
+  A.box_rows = kv.page_size % 128 == 0 && C::KT == 128 ? 128 : kv.page_size % 64 == 0 ? 64 : kv.page_size % 32 == 0 ? 32 : 16;
+  CUtensorMap tq, tk, tv;
+  EncodeTiled enc = encode_fn();
+  if (!enc || !page_map(&tk, kv.k, kv, A.Hkv, Dh, A.box_rows) || !page_map(&tv, kv.v, kv, A.Hkv, Dh, A.box_rows))
+    return cudaErrorInvalidValue;
+  // queries as (dim, head, row): a box is 64 dims x the group's heads x RP rows
+  const cuuint64_t dims[3] = {(cuuint64_t)Dh, (cuuint64_t)A.H, (cuuint64_t)A.pr.rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)Dh * 2, (cuuint64_t)A.H * Dh * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)A.G, (cuuint32_t)A.RP}, one[3] = {1, 1, 1};
+  if (enc(&tq, kv.dtype == WG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+          const_cast<void *>(q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cudaErrorInvalidValue;
+  const long long rpu = (long long)C::NT * A.RP;
+  const long long most = ((A.pr.rows + rpu - 1) / rpu + A.pr.batch) * A.Hkv;  // units there can be
+  const unsigned grid = (unsigned)(most < num_sms ? most : num_sms);
+  return launch_pdl(kern, dim3(grid), C::kThreads, C::kSmem, s, pdl, tq, tk, tv, A);
+}
+
+}  // namespace
+
+bool paged_prompt_supported(const PagedRows &rows, int H, int Hkv, int num_sms) {
+  (void)num_sms;
+  const int G = H / Hkv;
+  return G <= 128 && (long long)rows.rows / rows.batch * G >= 64;
+}
+
+cudaError_t launch_paged_prompt(const void *q, const PagedRows &rows, int H, int Hkv, int Dh, const wg_paged_kv &kv,
+                                int window, int sinks, void *out, unsigned *flags, int num_sms, cudaStream_t s,
+                                bool pdl) {
+  PromptArgs A{};
+  A.pr = rows;
+  A.pt = PagedTable{kv.table, kv.max_pages, kv.num_pages, kv.page_size};
+  A.out = out;
+  A.v = kv.v;
+  A.row_stride = kv.row_stride ? kv.row_stride : Dh;
+  A.head_stride = kv.head_stride ? kv.head_stride : (int64_t)kv.page_size * Dh;
+  A.page_stride = kv.page_stride ? kv.page_stride : (int64_t)Hkv * kv.page_size * Dh;
+  A.H = H;
+  A.Hkv = Hkv;
+  A.G = H / Hkv;
+  A.RP = 128 / A.G;
+  A.window = window;
+  A.sinks = sinks;
+  A.flags = flags;
+#define WG_PROMPT(T)                                                       \
+  if (Dh == 64) return prompt_t<T, 64>(q, A, kv, num_sms, s, pdl);   \
+  if (Dh == 128) return prompt_t<T, 128>(q, A, kv, num_sms, s, pdl); \
+  return prompt_t<T, 256>(q, A, kv, num_sms, s, pdl)
+  if (kv.dtype == WG_F16) {
+    WG_PROMPT(__half);
+  }
+  WG_PROMPT(__nv_bfloat16);
+#undef WG_PROMPT
+}
+
+}  // namespace wg
