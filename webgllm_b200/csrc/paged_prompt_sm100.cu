@@ -21,7 +21,7 @@
 //                while one's softmax runs, the other's products do;
 //   one warp     loads: Q by one 3-D TMA box a tile and 64 dims, K and V by the
 //                boxes of pages into a ring of stages;
-//   one warp     cleans V tiles that not every row sees in full: rows that no
+//   two warps    clean V tiles that not every row sees in full: rows that no
 //                row sees become zeros (their P is 0, but 0 times what a page
 //                holds there need not be), and infinities or NaN in the others
 //                are set aside (P = 0 must not meet them) and added at the end
@@ -53,7 +53,12 @@ struct PromptCfg {
   static constexpr int kStageBytes = KT * Dh * 2;  // K or V of a key tile
   static constexpr int kStages = (224 * 1024 - NT * kQBytes) / kStageBytes > 8 ? 8
                                  : (224 * 1024 - NT * kQBytes) / kStageBytes;
-  static constexpr int kThreads = (4 * NT + 3) * 32;
+  static constexpr int kThreads = (4 * NT + 4) * 32;
+  // Registers a thread: two softmax warpgroups and one of the other warps
+  // share what the launch got (384 x 168); with one tile 256 threads have 255.
+  static constexpr bool kSplitRegs = NT == 2;
+  static constexpr int kLaunchRegs = 168, kSoftRegs = 208, kHelpRegs = 88;
+  static_assert(!kSplitRegs || 256 * kSoftRegs + 128 * kHelpRegs <= kThreads * kLaunchRegs, "register split");
   static constexpr int kSmem = 1024 + NT * kQBytes + kStages * kStageBytes;
   static constexpr int kOCol = 256;  // tensor memory: scores at [0, 256), O after them
   static constexpr int kSCol = NT == 2 ? 128 : 64;  // columns between the two score buffers
@@ -136,16 +141,60 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Bits [a, b) of a 32-bit word (a, b clamped to 0 .. 32).
+__device__ __forceinline__ uint32_t bit_range(int a, int b) {
+  a = max(0, min(a, 32));
+  b = max(0, min(b, 32));
+  const uint32_t below_b = b >= 32 ? 0xFFFFFFFFu : (1u << b) - 1;
+  const uint32_t below_a = a >= 32 ? 0xFFFFFFFFu : (1u << a) - 1;
+  return below_b & ~below_a;
+}
+
 struct Unit : KeySpan {
   int b, hk, r0, n, p;
   int i0;  // first row of its NT tiles
 };
 
 // The units in order: sequence, then the rows from the last to the first, then
-// the KV head. Each role of a CTA walks the same ones.
+// the KV head; dealt to the CTAs in rounds, every other round backwards (the
+// units of a sequence get shorter, so a fixed order would give the first CTA
+// the longest of every round: 1.3x the mean). Each role of a CTA walks the
+// same ones.
 struct UnitWalk {
-  int b = 0;
+  int b = 0, round = 0;
   long long base = 0;
+  __device__ long long next() {
+    const long long item = (long long)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    round++;
+    return item;
+  }
   __device__ bool get(const PromptArgs &A, long long item, int rows_per_unit, int KT, Unit &u) {
     for (; b < A.pr.batch; b++) {
       seq_rows(A.pr, b, u.r0, u.n);
@@ -182,7 +231,7 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
       pv_done;
   __shared__ uint32_t tmem_slot;
   __shared__ int held[kHeldRing];
-  __shared__ int odd[kOddRing][kOddMax + 2];  // [0]: how many, then the tiles
+  __shared__ int odd[kOddRing][2][kOddMax + 2];  // of each half's warp: how many, then the tiles
   __shared__ int aborted;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int w_mma = 4 * NT, w_load = 4 * NT + 1;
@@ -196,7 +245,7 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
-    for (int i = 0; i < kHeldRing; i++) mbar_init(&v_ready[i], 1);
+    for (int i = 0; i < kHeldRing; i++) mbar_init(&v_ready[i], 2);
     for (int i = 0; i < 2; i++) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
@@ -238,211 +287,228 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
 
   UnitWalk walk;
   Unit u;
-  if (warp == w_load) {
-    // ---- loads ----
-    const int nb = KT / A.box_rows, nops = nb * kBlk;
-    const int box = lane % nb, blk = lane / nb;
-    const uint32_t box_bytes = (uint32_t)A.box_rows * 128;
-    const int groups = A.box_rows / 16, gmask = (1 << groups) - 1;
-    int stage = 0, phase = 0, nu = 0, nt = 0;
-    for (long long item = blockIdx.x; walk.get(A, item, rows_per_unit, KT, u); item += gridDim.x, nu++) {
-      wait(&q_empty, (nu & 1) ^ 1);
-      if (lane == 0) {
-        mbar_expect_tx(&q_full, (uint32_t)(NT * kBlk * A.G * A.RP * 128));
-        for (int t = 0; t < NT; t++)
-          for (int i = 0; i < kBlk; i++)
-            tma_load_3d(smem + t * C::kQBytes + i * 16384, &tm_q, i * 64, u.hk * A.G, u.r0 + u.i0 + t * A.RP, &q_full);
-      }
-      const int32_t *row = A.pt.table + (size_t)u.b * A.pt.max_pages;
-      auto entry = [&](int t, int &key, bool &seen) {
-        key = tile_key(u, t) + box * A.box_rows;
-        seen = lane < nops && key < u.hi && (key < u.se || key + A.box_rows > u.ws);
-        return seen ? row[key / A.pt.page_size] : -1;
-      };
-      int key, key_next = 0;
-      bool seen, seen_next = false;
-      int page = entry(0, key, seen), page_next = -1;
-      for (int t = 0; t < u.nt; t++, nt++) {
-        if (t + 1 < u.nt) page_next = entry(t + 1, key_next, seen_next);
-        const bool ok = seen && page >= 0 && page < A.pt.num_pages;
-        if (seen && !ok) raise_flag(A.flags, kFlagBadArgument);
-        const unsigned loaded = __ballot_sync(0xffffffffu, ok && lane < nb);
+  if (warp >= 4 * NT) {
+    if constexpr (C::kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kHelpRegs));
+    if (warp == w_load) {
+      // ---- loads ----
+      const int nb = KT / A.box_rows, nops = nb * kBlk;
+      const int box = lane % nb, blk = lane / nb;
+      const uint32_t box_bytes = (uint32_t)A.box_rows * 128;
+      const int groups = A.box_rows / 16, gmask = (1 << groups) - 1;
+      int stage = 0, phase = 0, nu = 0, nt = 0;
+      for (; walk.get(A, walk.next(), rows_per_unit, KT, u); nu++) {
+        wait(&q_empty, (nu & 1) ^ 1);
+        if (lane == 0) {
+          mbar_expect_tx(&q_full, (uint32_t)(NT * kBlk * A.G * A.RP * 128));
+          for (int t = 0; t < NT; t++)
+            for (int i = 0; i < kBlk; i++)
+              tma_load_3d(smem + t * C::kQBytes + i * 16384, &tm_q, i * 64, u.hk * A.G, u.r0 + u.i0 + t * A.RP, &q_full);
+        }
+        const int32_t *row = A.pt.table + (size_t)u.b * A.pt.max_pages;
+        auto entry = [&](int t, int &key, bool &seen) {
+          key = tile_key(u, t) + box * A.box_rows;
+          seen = lane < nops && key < u.hi && (key < u.se || key + A.box_rows > u.ws);
+          return seen ? row[key / A.pt.page_size] : -1;
+        };
+        int key, key_next = 0;
+        bool seen, seen_next = false;
+        int page = entry(0, key, seen), page_next = -1;
+        for (int t = 0; t < u.nt; t++, nt++) {
+          if (t + 1 < u.nt) page_next = entry(t + 1, key_next, seen_next);
+          const bool ok = seen && page >= 0 && page < A.pt.num_pages;
+          if (seen && !ok) raise_flag(A.flags, kFlagBadArgument);
+          const unsigned loaded = __ballot_sync(0xffffffffu, ok && lane < nb);
 #pragma unroll
-        for (int kv = 0; kv < 2; kv++) {  // K, then V
-          wait(&kv_empty[stage], phase ^ 1);
-          if (lane == 0) {
-            if (kv == 0) {
-              int m = 0;
-              for (int i = 0; i < nb; i++)
-                if (loaded >> i & 1) m |= gmask << (i * groups);
-              held[nt % kHeldRing] = m;
+          for (int kv = 0; kv < 2; kv++) {  // K, then V
+            wait(&kv_empty[stage], phase ^ 1);
+            if (lane == 0) {
+              if (kv == 0) {
+                int m = 0;
+                for (int i = 0; i < nb; i++)
+                  if (loaded >> i & 1) m |= gmask << (i * groups);
+                held[nt % kHeldRing] = m;
+              }
+              mbar_expect_tx(&kv_full[stage], (uint32_t)__popc(loaded) * box_bytes * kBlk);
             }
-            mbar_expect_tx(&kv_full[stage], (uint32_t)__popc(loaded) * box_bytes * kBlk);
+            __syncwarp();
+            if (ok)
+              tma_load_4d(ring + (size_t)stage * C::kStageBytes + blk * kBlkBytes + box * box_bytes, kv ? &tm_v : &tm_k,
+                          blk * 64, key % A.pt.page_size, u.hk, page, &kv_full[stage]);
+            if (++stage == S) stage = 0, phase ^= 1;
           }
-          __syncwarp();
-          if (ok)
-            tma_load_4d(ring + (size_t)stage * C::kStageBytes + blk * kBlkBytes + box * box_bytes, kv ? &tm_v : &tm_k,
-                        blk * 64, key % A.pt.page_size, u.hk, page, &kv_full[stage]);
+          page = page_next;
+          key = key_next;
+          seen = seen_next;
+        }
+      }
+      // after a wait that ran out, no copy may still be on its way when the CTA exits
+      __syncwarp();
+      if (*(volatile int *)&aborted && lane == 0) {
+        for (int i = 0; i < S; i++) {
+          mbar_wait_bounded(&kv_full[stage], phase ^ 1, A.flags);
           if (++stage == S) stage = 0, phase ^= 1;
         }
-        page = page_next;
-        key = key_next;
-        seen = seen_next;
+        if (nu) mbar_wait_bounded(&q_full, (nu - 1) & 1, A.flags);
       }
-    }
-    // after a wait that ran out, no copy may still be on its way when the CTA exits
-    __syncwarp();
-    if (*(volatile int *)&aborted && lane == 0) {
-      for (int i = 0; i < S; i++) {
-        mbar_wait_bounded(&kv_full[stage], phase ^ 1, A.flags);
-        if (++stage == S) stage = 0, phase ^= 1;
-      }
-      if (nu) mbar_wait_bounded(&q_full, (nu - 1) & 1, A.flags);
-    }
-  } else if (warp == w_mma) {
-    // ---- products ----
-    if (lane == 0) {
-      constexpr uint32_t qk_desc = instr_desc<T>(KT, false), pv_desc = instr_desc<T>(Dh, true);
-      int stage = 0, phase = 0, nu = 0, np = 0;
-      auto step = [&](int &s, int &ph) {
-        if (++s == S) s = 0, ph ^= 1;
-      };
-      // S_x = Q_t K^T
-      auto qk = [&](int t, int x, int st) {
-        const uint32_t q = smem_u32(smem) + t * C::kQBytes, k = smem_u32(ring) + st * C::kStageBytes;
+    } else if (warp == w_mma) {
+      // ---- products ----
+      if (lane == 0) {
+        constexpr uint32_t qk_desc = instr_desc<T>(KT, false), pv_desc = instr_desc<T>(Dh, true);
+        int stage = 0, phase = 0, nu = 0, np = 0;
+        auto step = [&](int &s, int &ph) {
+          if (++s == S) s = 0, ph ^= 1;
+        };
+        // S_x = Q_t K^T
+        auto qk = [&](int t, int x, int st) {
+          const uint32_t q = smem_u32(smem) + t * C::kQBytes, k = smem_u32(ring) + st * C::kStageBytes;
 #pragma unroll
-        for (int kk = 0; kk < Dh / 16; kk++)
-          mma_ss(tmem + x * C::kSCol, smem_desc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16),
-                 smem_desc(k + (kk >> 2) * kBlkBytes + (kk & 3) * 32, 16), qk_desc, kk > 0);
-      };
-      auto pv = [&](int t, int x, int st, bool first) {
-        const uint32_t v = smem_u32(ring) + st * C::kStageBytes;
+          for (int kk = 0; kk < Dh / 16; kk++)
+            mma_ss(tmem + x * C::kSCol, smem_desc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16),
+                   smem_desc(k + (kk >> 2) * kBlkBytes + (kk & 3) * 32, 16), qk_desc, kk > 0);
+        };
+        auto pv = [&](int t, int x, int st, bool first) {
+          const uint32_t v = smem_u32(ring) + st * C::kStageBytes;
 #pragma unroll
-        for (int kk = 0; kk < KT / 16; kk++)
-          mma_ts(tmem + C::kOCol + t * Dh, tmem + x * C::kSCol + kk * 8, smem_desc(v + kk * 2048, kBlkBytes), pv_desc,
-                 !(first && kk == 0));
-      };
-      for (long long item = blockIdx.x; walk.get(A, item, rows_per_unit, KT, u); item += gridDim.x, nu++) {
-        wait(&q_full, nu & 1);
-        wait(&kv_full[stage], phase);  // K of tile 0
-        tc_after();
-        if constexpr (NT == 2) {
-          for (int t = 0; t < 2; t++) {
-            qk(t, t, stage);
-            tc_commit_to(&s_full[t]);
-          }
-          tc_commit_to(&kv_empty[stage]);
-          step(stage, phase);
-          for (int j = 0; j < u.nt; j++, np++) {
-            const int vs = stage;
-            step(stage, phase);
-            const bool more = j + 1 < u.nt;
-            if (!more) tc_commit_to(&q_empty);
-            wait(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
+          for (int kk = 0; kk < KT / 16; kk++)
+            mma_ts(tmem + C::kOCol + t * Dh, tmem + x * C::kSCol + kk * 8, smem_desc(v + kk * 2048, kBlkBytes), pv_desc,
+                   !(first && kk == 0));
+        };
+        for (; walk.get(A, walk.next(), rows_per_unit, KT, u); nu++) {
+          wait(&q_full, nu & 1);
+          wait(&kv_full[stage], phase);  // K of tile 0
+          tc_after();
+          if constexpr (NT == 2) {
             for (int t = 0; t < 2; t++) {
-              wait(&p_full[t], np & 1);
-              if (j == 0) wait(&o_empty[t], (nu & 1) ^ 1);
-              tc_after();
-              pv(t, t, vs, j == 0);
-              if (t == 1) tc_commit_to(&kv_empty[vs]);
-              if (!more) tc_commit_to(&o_full[t]);
-              if (more) {
-                if (t == 0) {
-                  wait(&kv_full[stage], phase);
-                  tc_after();
-                }
-                qk(t, t, stage);
-                tc_commit_to(&s_full[t]);
-                if (t == 1) tc_commit_to(&kv_empty[stage]);
-              }
+              qk(t, t, stage);
+              tc_commit_to(&s_full[t]);
             }
-            if (more) step(stage, phase);
-          }
-        } else {
-          // one tile of rows, two buffers of scores: S(j + 1) is made while S(j)
-          // is in softmax
-          qk(0, np & 1, stage);
-          tc_commit_to(&s_full[np & 1]);
-          tc_commit_to(&kv_empty[stage]);
-          step(stage, phase);
-          for (int j = 0; j < u.nt; j++, np++) {
-            const int vs = stage;
+            tc_commit_to(&kv_empty[stage]);
             step(stage, phase);
-            if (j + 1 < u.nt) {
-              wait(&kv_full[stage], phase);
-              tc_after();
-              qk(0, (np + 1) & 1, stage);
-              tc_commit_to(&s_full[(np + 1) & 1]);
-              tc_commit_to(&kv_empty[stage]);
+            for (int j = 0; j < u.nt; j++, np++) {
+              const int vs = stage;
               step(stage, phase);
-            } else {
-              tc_commit_to(&q_empty);
+              const bool more = j + 1 < u.nt;
+              if (!more) tc_commit_to(&q_empty);
+              wait(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
+              for (int t = 0; t < 2; t++) {
+                wait(&p_full[t], np & 1);
+                if (j == 0) wait(&o_empty[t], (nu & 1) ^ 1);
+                tc_after();
+                pv(t, t, vs, j == 0);
+                if (t == 1) tc_commit_to(&kv_empty[vs]);
+                if (!more) tc_commit_to(&o_full[t]);
+                if (more) {
+                  if (t == 0) {
+                    wait(&kv_full[stage], phase);
+                    tc_after();
+                  }
+                  qk(t, t, stage);
+                  tc_commit_to(&s_full[t]);
+                  if (t == 1) tc_commit_to(&kv_empty[stage]);
+                }
+              }
+              if (more) step(stage, phase);
             }
-            wait(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
-            wait(&p_full[np & 1], (np >> 1) & 1);
-            if (j == 0) wait(&o_empty[0], (nu & 1) ^ 1);
-            tc_after();
-            pv(0, np & 1, vs, j == 0);
-            tc_commit_to(&kv_empty[vs]);
-            tc_commit_to(&pv_done);
-            if (j + 1 == u.nt) tc_commit_to(&o_full[0]);
+          } else {
+            // one tile of rows, two buffers of scores: S(j + 1) is made while S(j)
+            // is in softmax
+            qk(0, np & 1, stage);
+            tc_commit_to(&s_full[np & 1]);
+            tc_commit_to(&kv_empty[stage]);
+            step(stage, phase);
+            for (int j = 0; j < u.nt; j++, np++) {
+              const int vs = stage;
+              step(stage, phase);
+              if (j + 1 < u.nt) {
+                wait(&kv_full[stage], phase);
+                tc_after();
+                qk(0, (np + 1) & 1, stage);
+                tc_commit_to(&s_full[(np + 1) & 1]);
+                tc_commit_to(&kv_empty[stage]);
+                step(stage, phase);
+              } else {
+                tc_commit_to(&q_empty);
+              }
+              wait(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
+              wait(&p_full[np & 1], (np >> 1) & 1);
+              if (j == 0) wait(&o_empty[0], (nu & 1) ^ 1);
+              tc_after();
+              pv(0, np & 1, vs, j == 0);
+              tc_commit_to(&kv_empty[vs]);
+              tc_commit_to(&pv_done);
+              if (j + 1 == u.nt) tc_commit_to(&o_full[0]);
+            }
           }
         }
       }
-    }
-  } else if (warp == w_load + 1) {
-    // ---- V tiles that some rows do not see in full ----
-    int stage = 0, phase = 0, nu = 0, nt = 0;
-    for (long long item = blockIdx.x; walk.get(A, item, rows_per_unit, KT, u); item += gridDim.x, nu++) {
-      int *list = odd[nu % kOddRing];
-      int nodd = 0;
-      for (int t = 0; t < u.nt; t++, nt++) {
-        if (++stage == S) stage = 0, phase ^= 1;  // past K
-        wait(&kv_full[stage], phase);
-        const int key0 = tile_key(u, t), m = held[nt % kHeldRing];
-        if (!open_tile(u, key0) || m != kAll) {
-          bool found = false;
-          uint8_t *v = ring + (size_t)stage * C::kStageBytes;
-          for (int i = lane; i < KT * (Dh / 8); i += 32) {
-            const int kr = i / (Dh / 8), ch = i - kr * (Dh / 8), key = key0 + kr;
-            uint4 *at =
-                reinterpret_cast<uint4 *>(v + (ch >> 3) * kBlkBytes + kr * 128 + (((ch & 7) ^ (kr & 7)) << 4));
-            if (key >= u.hi || (key >= u.se && key < u.ws) || !(m >> (kr >> 4) & 1)) {
-              *at = make_uint4(0, 0, 0, 0);
-            } else {
-              uint4 x = *at;
-              uint32_t w[4] = {x.x, x.y, x.z, x.w};
-              bool here = false;
+    } else {
+      // ---- V tiles that some rows do not see in full: two warps, half a tile each ----
+      const int half = warp - w_load - 1;
+      int stage = 0, phase = 0, nu = 0, nt = 0;
+      for (; walk.get(A, walk.next(), rows_per_unit, KT, u); nu++) {
+        int *list = odd[nu % kOddRing][half];
+        int nodd = 0;
+        for (int t = 0; t < u.nt; t++, nt++) {
+          if (++stage == S) stage = 0, phase ^= 1;  // past K
+          wait(&kv_full[stage], phase);
+          const int key0 = tile_key(u, t), m = held[nt % kHeldRing];
+          if (!open_tile(u, key0) || m != kAll) {
+            bool found = false;
+            uint8_t *v = ring + (size_t)stage * C::kStageBytes;
+            // 16-byte pieces of this warp's rows, eight in flight
+            constexpr int kPieces = KT / 2 * (Dh / 8), kPer = 8;
+            for (int i0 = lane; i0 < kPieces; i0 += 32 * kPer) {
+              uint4 x[kPer];
+              uint4 *at[kPer];
+              bool none[kPer];
 #pragma unroll
-              for (int e = 0; e < 4; e++) {
-                constexpr uint32_t ex = kNonfinite<T>;
-                if ((w[e] & ex) == ex) w[e] &= 0xFFFF0000u, here = true;
-                if ((w[e] >> 16 & ex) == ex) w[e] &= 0xFFFFu, here = true;
+              for (int e = 0; e < kPer; e++) {
+                const int i = i0 + 32 * e, kr = half * (KT / 2) + i / (Dh / 8), ch = i % (Dh / 8), key = key0 + kr;
+                at[e] = reinterpret_cast<uint4 *>(v + (ch >> 3) * kBlkBytes + kr * 128 + (((ch & 7) ^ (kr & 7)) << 4));
+                none[e] = key >= u.hi || (key >= u.se && key < u.ws) || !(m >> (kr >> 4) & 1);
+                x[e] = *at[e];
               }
-              if (here) *at = make_uint4(w[0], w[1], w[2], w[3]);
-              found |= here;
+#pragma unroll
+              for (int e = 0; e < kPer; e++) {
+                if (none[e]) {
+                  *at[e] = make_uint4(0, 0, 0, 0);
+                } else if (nonfinite2<T>(x[e].x) || nonfinite2<T>(x[e].y) || nonfinite2<T>(x[e].z) ||
+                           nonfinite2<T>(x[e].w)) {
+                  uint32_t w[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
+#pragma unroll
+                  for (int k = 0; k < 4; k++) {
+                    constexpr uint32_t ex = kNonfinite<T>;
+                    if ((w[k] & ex) == ex) w[k] &= 0xFFFF0000u;
+                    if ((w[k] >> 16 & ex) == ex) w[k] &= 0xFFFFu;
+                  }
+                  *at[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                  found = true;
+                }
+              }
+            }
+            static_assert(kPieces % (32 * kPer) == 0, "whole rounds");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            if (__any_sync(0xffffffffu, found) && nodd < kOddMax) {
+              if (lane == 0) list[1 + nodd] = t;
+              nodd++;
             }
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          if (__any_sync(0xffffffffu, found) && nodd < kOddMax) {
-            if (lane == 0) list[1 + nodd] = t;
-            nodd++;
-          }
+          if (t + 1 == u.nt && lane == 0) list[0] = nodd;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_ready[nt % kHeldRing]);
+          if (++stage == S) stage = 0, phase ^= 1;
         }
-        if (t + 1 == u.nt && lane == 0) list[0] = nodd;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_ready[nt % kHeldRing]);
-        if (++stage == S) stage = 0, phase ^= 1;
       }
     }
   } else {
     // ---- softmax: one row a thread ----
+    if constexpr (C::kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
     const int t = warp >> 2, m = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + lanes + C::kOCol + t * Dh;
     const int i_in = m / A.G, g = m - i_in * A.G;
     int nu = 0, np = 0;
-    for (long long item = blockIdx.x; walk.get(A, item, rows_per_unit, KT, u); item += gridDim.x, nu++) {
+    for (; walk.get(A, walk.next(), rows_per_unit, KT, u); nu++) {
       const int i = u.i0 + t * A.RP + i_in;
       const bool valid = i_in < A.RP && i < u.n;
       const int p = valid ? (int)max(-1LL, min((long long)u.p + i, 0x7ffffffeLL)) : -1;
@@ -458,15 +524,28 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
         tmem_wait_ld();
         const int key0 = tile_key(u, j), hm = held[np % kHeldRing];
         if (!open_tile(u, key0) || hm != kAll) {
+          // the row's keys of this tile: below its position and the sequence's
+          // end, inside the window or among the sinks, on a page that exists
+          const int end = min(p + 1, u.hi) - key0;
+          const int from = A.window > 0 ? (int)max(0LL, (long long)p - A.window + 1 - key0) : 0;
 #pragma unroll
-          for (int c = 0; c < KT; c++) {
-            const int key = key0 + c;
-            if (!(hm >> (c >> 4) & 1) || key >= u.hi || !sees_key(p, key, A.window, A.sinks)) s[c] = -INFINITY;
+          for (int w = 0; w < KT / 32; w++) {
+            uint32_t see = bit_range(from - 32 * w, end - 32 * w) |
+                           bit_range(0, min(end, min(A.sinks, 1 << 30) - key0) - 32 * w);
+            if (!(hm >> (2 * w) & 1)) see &= 0xFFFF0000u;
+            if (!(hm >> (2 * w + 1) & 1)) see &= 0xFFFFu;
+#pragma unroll
+            for (int c = 0; c < 32; c++)
+              if (!(see >> c & 1)) s[32 * w + c] = -INFINITY;
           }
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < KT; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+        for (int c = 4; c < KT; c += 8) {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            mx[e] = c + 4 + e < KT ? max3(mx[e], s[c + e], s[c + 4 + e]) : fmaxf(mx[e], s[c + e]);
+        }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
         const bool grow = top > ref + 8.0f || (ref == -INFINITY && top > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
@@ -493,20 +572,24 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
           }
         }
         const float sub = ref == -INFINITY ? 0.0f : ref;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t scale2 = pair(kLog2e, kLog2e), sub2 = pair(-sub, -sub);
+        uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < KT / 64; c++) {
           uint32_t r[32];
 #pragma unroll
           for (int e = 0; e < 32; e++) {
-            const float a = ex2(fmaf(s[c * 64 + 2 * e], kLog2e, -sub));
-            const float b = ex2(fmaf(s[c * 64 + 2 * e + 1], kLog2e, -sub));
-            sum[e & 3] += a + b;
+            const float2 v = unpair(fma2(pair(s[c * 64 + 2 * e], s[c * 64 + 2 * e + 1]), scale2, sub2));
+            const float a = ex2(v.x), b = ex2(v.y);
+            sum[e & 3] = add2(sum[e & 3], pair(a, b));
             r[e] = pack2<T>(a, b);
           }
           tmem_st32(s_addr + c * 32, r);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        {
+          const float2 v = unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+          l += v.x + v.y;
+        }
         tmem_wait_st();
         tc_before();
         __syncwarp();
@@ -515,8 +598,7 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
       // ---- the rows' results
       wait(&o_full[t], nu & 1);
       tc_after();
-      const int *list = odd[nu % kOddRing];
-      const int nodd = list[0];
+      const int nodd[2] = {odd[nu % kOddRing][0][0], odd[nu % kOddRing][1][0]};
       const float inv = ref == -INFINITY ? 0.0f : 1.0f / l;
       T *dst = reinterpret_cast<T *>(A.out) + ((size_t)(u.r0 + i) * A.H + u.hk * A.G + g) * Dh;
 #pragma unroll 1
@@ -524,11 +606,12 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
         float o[32];
         tmem_ld32(o_addr + c * 32, o);
         tmem_wait_ld();
-        if (nodd && valid) {
+        if ((nodd[0] | nodd[1]) && valid) {
           // infinities and NaN of V that this row does see
-          for (int k = 0; k < nodd; k++) {
-            const int key0 = tile_key(u, list[1 + k]);
-            for (int key = key0; key < key0 + KT; key++) {
+          for (int k = 0; k < nodd[0] + nodd[1]; k++) {
+            const int half = k >= nodd[0];
+            const int key0 = tile_key(u, odd[nu % kOddRing][half][1 + k - (half ? nodd[0] : 0)]) + half * (KT / 2);
+            for (int key = key0; key < key0 + KT / 2; key++) {
               if (key >= u.hi || !sees_key(p, key, A.window, A.sinks)) continue;
               const int page = A.pt.table[(size_t)u.b * A.pt.max_pages + key / A.pt.page_size];
               if (page < 0 || page >= A.pt.num_pages) continue;
@@ -580,6 +663,14 @@ cudaError_t prompt_t(const void *q, PromptArgs A, const wg_paged_kv &kv, int num
   auto kern = paged_prompt_kernel<T, Dh>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return e;
+  if constexpr (C::kSplitRegs) {
+    // the split needs what it was counted against
+    static const bool enough = [&] {
+      cudaFuncAttributes at;
+      return cudaFuncGetAttributes(&at, kern) == cudaSuccess && at.numRegs >= C::kLaunchRegs;
+    }();
+    if (!enough) return cudaErrorInvalidConfiguration;
+  }
   A.box_rows = kv.page_size % 128 == 0 && C::KT == 128 ? 128 : kv.page_size % 64 == 0 ? 64 : kv.page_size % 32 == 0 ? 32 : 16;
   CUtensorMap tq, tk, tv;
   EncodeTiled enc = encode_fn();
