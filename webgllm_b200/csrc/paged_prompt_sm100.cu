@@ -79,24 +79,39 @@ struct PromptArgs {
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ void tc_commit_to(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+// The issuing warp runs as one: every lane follows the same path and `lead`
+// (one lane, elected once) guards only the instruction itself, so that its
+// operands stay in uniform registers. Issued from a branch of a single lane
+// each product cost 100 cycles of operand moves: more than it runs for.
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void tc_commit_to(uint32_t bar, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(lead)
+      : "memory");
 }
 
 // D (+)= A B with A and B in shared memory, or A in tensor memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                                       uint32_t lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                                       uint32_t lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
 
@@ -140,6 +155,31 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// mbar_wait_bounded as one piece of code (the compiler sees no loop whose trips
+// could differ between lanes): false after about `cycles`.
+constexpr long long kWaitCycles = 2000000000LL;
+__device__ __forceinline__ bool wait_one_path(uint64_t *bar, uint32_t parity, long long cycles) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u64 t0, t1;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "mov.u64 t0, %%clock64;\n\t"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "mov.u64 t1, %%clock64;\n\t"
+      "sub.u64 t1, t1, t0;\n\t"
+      "setp.lt.u64 q, t1, %3;\n\t"
+      "@q bra AGAIN;\n\t"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "l"(cycles)
+      : "memory");
+  return ok != 0;
+}
 
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
@@ -274,8 +314,10 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
   const uint32_t tmem = tmem_slot;
 
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    if (*(volatile int *)&aborted) return;
-    if (!mbar_wait_bounded(bar, parity, A.flags)) *(volatile int *)&aborted = 1;
+    if (!wait_one_path(bar, parity, *(volatile int *)&aborted ? 0 : kWaitCycles)) {
+      raise_flag(A.flags, kFlagTimeout);
+      *(volatile int *)&aborted = 1;
+    }
   };
   // whether every row of the unit sees every key of tile t
   auto open_tile = [&](const Unit &u, int key0) {
@@ -352,7 +394,15 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
       }
     } else if (warp == w_mma) {
       // ---- products ----
-      if (lane == 0) {
+      {
+        const uint32_t lead = elect_lane();
+        const uint32_t smem0 = __shfl_sync(0xffffffffu, smem_u32(smem), 0), ring0 = smem0 + NT * C::kQBytes;
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        auto commit = [&](uint64_t *bar) { tc_commit_to(smem_u32(bar), lead); };
+        auto wait1 = [&](uint64_t *bar, uint32_t parity) {
+          wait(bar, parity);
+          __syncwarp();
+        };
         constexpr uint32_t qk_desc = instr_desc<T>(KT, false), pv_desc = instr_desc<T>(Dh, true);
         int stage = 0, phase = 0, nu = 0, np = 0;
         auto step = [&](int &s, int &ph) {
@@ -360,51 +410,52 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
         };
         // S_x = Q_t K^T
         auto qk = [&](int t, int x, int st) {
-          const uint32_t q = smem_u32(smem) + t * C::kQBytes, k = smem_u32(ring) + st * C::kStageBytes;
+          const uint32_t q = smem0 + t * C::kQBytes, k = ring0 + st * C::kStageBytes;
 #pragma unroll
           for (int kk = 0; kk < Dh / 16; kk++)
-            mma_ss(tmem + x * C::kSCol, smem_desc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16),
-                   smem_desc(k + (kk >> 2) * kBlkBytes + (kk & 3) * 32, 16), qk_desc, kk > 0);
+            mma_ss(tm + x * C::kSCol, smem_desc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16),
+                   smem_desc(k + (kk >> 2) * kBlkBytes + (kk & 3) * 32, 16), qk_desc, kk > 0, lead);
         };
         auto pv = [&](int t, int x, int st, bool first) {
-          const uint32_t v = smem_u32(ring) + st * C::kStageBytes;
+          const uint32_t v = ring0 + st * C::kStageBytes;
 #pragma unroll
           for (int kk = 0; kk < KT / 16; kk++)
-            mma_ts(tmem + C::kOCol + t * Dh, tmem + x * C::kSCol + kk * 8, smem_desc(v + kk * 2048, kBlkBytes), pv_desc,
-                   !(first && kk == 0));
+            mma_ts(tm + C::kOCol + t * Dh, tm + x * C::kSCol + kk * 8, smem_desc(v + kk * 2048, kBlkBytes), pv_desc,
+                   !(first && kk == 0), lead);
         };
-        for (; walk.get(A, walk.next(), rows_per_unit, KT, u); nu++) {
-          wait(&q_full, nu & 1);
-          wait(&kv_full[stage], phase);  // K of tile 0
+        for (; __shfl_sync(0xffffffffu, walk.get(A, walk.next(), rows_per_unit, KT, u), 0); nu++) {
+          u.nt = __shfl_sync(0xffffffffu, u.nt, 0);
+          wait1(&q_full, nu & 1);
+          wait1(&kv_full[stage], phase);  // K of tile 0
           tc_after();
           if constexpr (NT == 2) {
             for (int t = 0; t < 2; t++) {
               qk(t, t, stage);
-              tc_commit_to(&s_full[t]);
+              commit(&s_full[t]);
             }
-            tc_commit_to(&kv_empty[stage]);
+            commit(&kv_empty[stage]);
             step(stage, phase);
             for (int j = 0; j < u.nt; j++, np++) {
               const int vs = stage;
               step(stage, phase);
               const bool more = j + 1 < u.nt;
-              if (!more) tc_commit_to(&q_empty);
-              wait(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
+              if (!more) commit(&q_empty);
+              wait1(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
               for (int t = 0; t < 2; t++) {
-                wait(&p_full[t], np & 1);
-                if (j == 0) wait(&o_empty[t], (nu & 1) ^ 1);
+                wait1(&p_full[t], np & 1);
+                if (j == 0) wait1(&o_empty[t], (nu & 1) ^ 1);
                 tc_after();
                 pv(t, t, vs, j == 0);
-                if (t == 1) tc_commit_to(&kv_empty[vs]);
-                if (!more) tc_commit_to(&o_full[t]);
+                if (t == 1) commit(&kv_empty[vs]);
+                if (!more) commit(&o_full[t]);
                 if (more) {
                   if (t == 0) {
-                    wait(&kv_full[stage], phase);
+                    wait1(&kv_full[stage], phase);
                     tc_after();
                   }
                   qk(t, t, stage);
-                  tc_commit_to(&s_full[t]);
-                  if (t == 1) tc_commit_to(&kv_empty[stage]);
+                  commit(&s_full[t]);
+                  if (t == 1) commit(&kv_empty[stage]);
                 }
               }
               if (more) step(stage, phase);
@@ -413,30 +464,30 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
             // one tile of rows, two buffers of scores: S(j + 1) is made while S(j)
             // is in softmax
             qk(0, np & 1, stage);
-            tc_commit_to(&s_full[np & 1]);
-            tc_commit_to(&kv_empty[stage]);
+            commit(&s_full[np & 1]);
+            commit(&kv_empty[stage]);
             step(stage, phase);
             for (int j = 0; j < u.nt; j++, np++) {
               const int vs = stage;
               step(stage, phase);
               if (j + 1 < u.nt) {
-                wait(&kv_full[stage], phase);
+                wait1(&kv_full[stage], phase);
                 tc_after();
                 qk(0, (np + 1) & 1, stage);
-                tc_commit_to(&s_full[(np + 1) & 1]);
-                tc_commit_to(&kv_empty[stage]);
+                commit(&s_full[(np + 1) & 1]);
+                commit(&kv_empty[stage]);
                 step(stage, phase);
               } else {
-                tc_commit_to(&q_empty);
+                commit(&q_empty);
               }
-              wait(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
-              wait(&p_full[np & 1], (np >> 1) & 1);
-              if (j == 0) wait(&o_empty[0], (nu & 1) ^ 1);
+              wait1(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
+              wait1(&p_full[np & 1], (np >> 1) & 1);
+              if (j == 0) wait1(&o_empty[0], (nu & 1) ^ 1);
               tc_after();
               pv(0, np & 1, vs, j == 0);
-              tc_commit_to(&kv_empty[vs]);
-              tc_commit_to(&pv_done);
-              if (j + 1 == u.nt) tc_commit_to(&o_full[0]);
+              commit(&kv_empty[vs]);
+              commit(&pv_done);
+              if (j + 1 == u.nt) commit(&o_full[0]);
             }
           }
         }
