@@ -41,27 +41,33 @@ namespace {
 
 // Entries by key tile (not by stage: a stage carries K of one round and V of
 // another): which page boxes of the tile were loaded; whether its V is clean.
-constexpr int kHeldRing = 8;
+constexpr int kHeldRing = 16;
 constexpr int kOddRing = 8, kOddMax = 14;
 
 template <int Dh_>
 struct PromptCfg {
   static constexpr int Dh = Dh_;
   static constexpr int NT = Dh == 256 ? 1 : 2;   // query tiles of a CTA
-  static constexpr int KT = Dh == 256 ? 64 : 128;  // keys of a tile
+  static constexpr int KT = Dh == 128 ? 128 : 64;  // keys of a tile
+  static constexpr int NB = Dh == 128 ? 1 : 2;     // score buffers of a query tile
   static constexpr int kQBytes = 128 * Dh * 2;     // one query tile
   static constexpr int kStageBytes = KT * Dh * 2;  // K or V of a key tile
-  static constexpr int kStages = (224 * 1024 - NT * kQBytes) / kStageBytes > 8 ? 8
-                                 : (224 * 1024 - NT * kQBytes) / kStageBytes;
-  static constexpr int kThreads = (4 * NT + 4) * 32;
-  // Registers a thread: two softmax warpgroups and one of the other warps
-  // share what the launch got (384 x 168); with one tile 256 threads have 255.
+  static constexpr int kFit = (224 * 1024 - NT * kQBytes) / kStageBytes;
+  static constexpr int kStages = kFit > 12 ? 12 : kFit;
+  static constexpr int NH = KT / 64;  // parts of a tile that softmax hands over on its own
+  static constexpr int kSoftWarps = 4 * NT;
+  static constexpr int kThreads = (kSoftWarps + 4) * 32;
+  // Registers a thread: two softmax warpgroups and the four other warps share
+  // what the launch got (384 x 168); with one tile 256 threads have 255.
   static constexpr bool kSplitRegs = NT == 2;
   static constexpr int kLaunchRegs = 168, kSoftRegs = 208, kHelpRegs = 88;
   static_assert(!kSplitRegs || 256 * kSoftRegs + 128 * kHelpRegs <= kThreads * kLaunchRegs, "register split");
+  // score buffer of the np-th tile of a CTA, and its round's parity
+  static __device__ int buffer(int np) { return NB == 2 ? np & 1 : 0; }
+  static __device__ int parity(int np) { return NB == 2 ? (np >> 1) & 1 : np & 1; }
+  static __device__ int score_col(int t, int x) { return (t * NB + x) * KT; }
   static constexpr int kSmem = 1024 + NT * kQBytes + kStages * kStageBytes;
   static constexpr int kOCol = 256;  // tensor memory: scores at [0, 256), O after them
-  static constexpr int kSCol = NT == 2 ? 128 : 64;  // columns between the two score buffers
 };
 
 struct PromptArgs {
@@ -151,6 +157,26 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float *v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -267,14 +293,14 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *ring = smem + NT * C::kQBytes;
-  __shared__ uint64_t q_full, q_empty, kv_full[S], kv_empty[S], v_ready[kHeldRing], s_full[2], p_full[2], o_full[2], o_empty[2],
-      pv_done;
+  __shared__ uint64_t q_full, q_empty, kv_full[S], kv_empty[S], v_ready[kHeldRing], s_full[2][2], p_full[2][2], o_full[2],
+      o_empty[2], pv_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int held[kHeldRing];
-  __shared__ int odd[kOddRing][2][kOddMax + 2];  // of each half's warp: how many, then the tiles
+  __shared__ int odd[kOddRing][2][kOddMax + 2];  // of each half: how many, then the tiles
   __shared__ int aborted;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int w_mma = 4 * NT, w_load = 4 * NT + 1;
+  const int w_mma = C::kSoftWarps, w_load = w_mma + 1;
   const int rows_per_unit = NT * A.RP;
   constexpr int kAll = (1 << (KT / 16)) - 1;
 
@@ -287,12 +313,14 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
     }
     for (int i = 0; i < kHeldRing; i++) mbar_init(&v_ready[i], 2);
     for (int i = 0; i < 2; i++) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      for (int x = 0; x < 2; x++) {
+        mbar_init(&s_full[i][x], 1);
+        mbar_init(&p_full[i][x], 4);
+      }
       mbar_init(&o_full[i], 1);
       mbar_init(&o_empty[i], 4);
+      mbar_init(&pv_done[i], 1);
     }
-    mbar_init(&pv_done, 1);
     fence_mbar_init();
     aborted = 0;
   }
@@ -314,6 +342,7 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
   const uint32_t tmem = tmem_slot;
 
   auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return;
     if (!wait_one_path(bar, parity, *(volatile int *)&aborted ? 0 : kWaitCycles)) {
       raise_flag(A.flags, kFlagTimeout);
       *(volatile int *)&aborted = 1;
@@ -329,7 +358,7 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
 
   UnitWalk walk;
   Unit u;
-  if (warp >= 4 * NT) {
+  if (warp >= C::kSoftWarps) {
     if constexpr (C::kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kHelpRegs));
     if (warp == w_load) {
       // ---- loads ----
@@ -408,87 +437,58 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
         auto step = [&](int &s, int &ph) {
           if (++s == S) s = 0, ph ^= 1;
         };
-        // S_x = Q_t K^T
+        // S_t = Q_t K^T into score buffer x of tile t; O_t += P_t V
         auto qk = [&](int t, int x, int st) {
           const uint32_t q = smem0 + t * C::kQBytes, k = ring0 + st * C::kStageBytes;
 #pragma unroll
           for (int kk = 0; kk < Dh / 16; kk++)
-            mma_ss(tm + x * C::kSCol, smem_desc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16),
+            mma_ss(tm + C::score_col(t, x), smem_desc(q + (kk >> 2) * 16384 + (kk & 3) * 32, 16),
                    smem_desc(k + (kk >> 2) * kBlkBytes + (kk & 3) * 32, 16), qk_desc, kk > 0, lead);
+          commit(&s_full[t][x]);
+          if (t == NT - 1) commit(&kv_empty[st]);
         };
-        auto pv = [&](int t, int x, int st, bool first) {
+        auto pv = [&](int t, int x, int part, int st, bool first) {
           const uint32_t v = ring0 + st * C::kStageBytes;
 #pragma unroll
-          for (int kk = 0; kk < KT / 16; kk++)
-            mma_ts(tm + C::kOCol + t * Dh, tm + x * C::kSCol + kk * 8, smem_desc(v + kk * 2048, kBlkBytes), pv_desc,
-                   !(first && kk == 0), lead);
+          for (int kk = 4 * part; kk < 4 * part + 4; kk++)
+            mma_ts(tm + C::kOCol + t * Dh, tm + C::score_col(t, x) + kk * 8, smem_desc(v + kk * 2048, kBlkBytes),
+                   pv_desc, !(first && kk == 0), lead);
+          if (t == NT - 1 && part == C::NH - 1) commit(&kv_empty[st]);
+          if (part < C::NH - 1 || C::NB == 2) commit(&pv_done[t]);
         };
         for (; __shfl_sync(0xffffffffu, walk.get(A, walk.next(), rows_per_unit, KT, u), 0); nu++) {
           u.nt = __shfl_sync(0xffffffffu, u.nt, 0);
           wait1(&q_full, nu & 1);
           wait1(&kv_full[stage], phase);  // K of tile 0
           tc_after();
-          if constexpr (NT == 2) {
-            for (int t = 0; t < 2; t++) {
-              qk(t, t, stage);
-              commit(&s_full[t]);
-            }
-            commit(&kv_empty[stage]);
+#pragma unroll
+          for (int t = 0; t < NT; t++) qk(t, C::buffer(np), stage);
+          step(stage, phase);
+          for (int j = 0; j < u.nt; j++, np++) {
+            const int vs = stage, x = C::buffer(np);
             step(stage, phase);
-            for (int j = 0; j < u.nt; j++, np++) {
-              const int vs = stage;
-              step(stage, phase);
-              const bool more = j + 1 < u.nt;
-              if (!more) commit(&q_empty);
-              wait1(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
-              for (int t = 0; t < 2; t++) {
-                wait1(&p_full[t], np & 1);
-                if (j == 0) wait1(&o_empty[t], (nu & 1) ^ 1);
+            const bool more = j + 1 < u.nt;
+            if (more)
+              wait1(&kv_full[stage], phase);  // K of tile j + 1
+            else
+              commit(&q_empty);
+            if (C::NB == 1) wait1(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
+            tc_after();
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              if (C::NB == 2 && more) qk(t, x ^ 1, stage);
+              if (C::NB == 2 && t == 0) wait1(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
+              if (j == 0) wait1(&o_empty[t], (nu & 1) ^ 1);
+#pragma unroll
+              for (int part = 0; part < C::NH; part++) {
+                wait1(&p_full[t][C::NH == 1 ? x : part], C::parity(np));
                 tc_after();
-                pv(t, t, vs, j == 0);
-                if (t == 1) commit(&kv_empty[vs]);
-                if (!more) commit(&o_full[t]);
-                if (more) {
-                  if (t == 0) {
-                    wait1(&kv_full[stage], phase);
-                    tc_after();
-                  }
-                  qk(t, t, stage);
-                  commit(&s_full[t]);
-                  if (t == 1) commit(&kv_empty[stage]);
-                }
+                pv(t, x, part, vs, j == 0 && part == 0);
               }
-              if (more) step(stage, phase);
+              if (!more) commit(&o_full[t]);
+              if (C::NB == 1 && more) qk(t, x, stage);
             }
-          } else {
-            // one tile of rows, two buffers of scores: S(j + 1) is made while S(j)
-            // is in softmax
-            qk(0, np & 1, stage);
-            commit(&s_full[np & 1]);
-            commit(&kv_empty[stage]);
-            step(stage, phase);
-            for (int j = 0; j < u.nt; j++, np++) {
-              const int vs = stage;
-              step(stage, phase);
-              if (j + 1 < u.nt) {
-                wait1(&kv_full[stage], phase);
-                tc_after();
-                qk(0, (np + 1) & 1, stage);
-                commit(&s_full[(np + 1) & 1]);
-                commit(&kv_empty[stage]);
-                step(stage, phase);
-              } else {
-                commit(&q_empty);
-              }
-              wait1(&v_ready[np % kHeldRing], (np / kHeldRing) & 1);
-              wait1(&p_full[np & 1], (np >> 1) & 1);
-              if (j == 0) wait1(&o_empty[0], (nu & 1) ^ 1);
-              tc_after();
-              pv(0, np & 1, vs, j == 0);
-              commit(&kv_empty[vs]);
-              commit(&pv_done);
-              if (j + 1 == u.nt) commit(&o_full[0]);
-            }
+            if (more) step(stage, phase);
           }
         }
       }
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
           if (!open_tile(u, key0) || m != kAll) {
             bool found = false;
             uint8_t *v = ring + (size_t)stage * C::kStageBytes;
-            // 16-byte pieces of this warp's rows, eight in flight
+            // 16-byte pieces, eight a lane in flight
             constexpr int kPieces = KT / 2 * (Dh / 8), kPer = 8;
             for (int i0 = lane; i0 < kPieces; i0 += 32 * kPer) {
               uint4 x[kPer];
@@ -514,7 +514,8 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
               bool none[kPer];
 #pragma unroll
               for (int e = 0; e < kPer; e++) {
-                const int i = i0 + 32 * e, kr = half * (KT / 2) + i / (Dh / 8), ch = i % (Dh / 8), key = key0 + kr;
+                const int i = i0 + 32 * e, kr = half * (KT / 2) + i / (Dh / 8), ch = i % (Dh / 8),
+                          key = key0 + kr;
                 at[e] = reinterpret_cast<uint4 *>(v + (ch >> 3) * kBlkBytes + kr * 128 + (((ch & 7) ^ (kr & 7)) << 4));
                 none[e] = key >= u.hi || (key >= u.se && key < u.ws) || !(m >> (kr >> 4) & 1);
                 x[e] = *at[e];
@@ -563,18 +564,25 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
       const int i = u.i0 + t * A.RP + i_in;
       const bool valid = i_in < A.RP && i < u.n;
       const int p = valid ? (int)max(-1LL, min((long long)u.p + i, 0x7ffffffeLL)) : -1;
+      // tiles whose keys every row of the unit sees: key0 <= open_to, and past the
+      // last row's window start or all sinks
+      const long long first = (long long)u.p + u.i0, last = (long long)u.p + min(u.n, u.i0 + rows_per_unit) - 1;
+      const int open_to = (int)max(-1LL, min(first, 0x7ffffffeLL) - (KT - 1));
+      const int open_from = A.window > 0 ? (int)max(0LL, min(last, 0x7ffffffeLL) - A.window + 1) : 0;
+      const int open_sinks = A.sinks - (KT - 1);
       float ref = -INFINITY, l = 0.0f;  // the reference maximum (log2 units) and the row sum over it
       for (int j = 0; j < u.nt; j++, np++) {
-        const int x = NT == 2 ? t : np & 1;
-        const uint32_t s_addr = tmem + lanes + x * C::kSCol;
-        wait(&s_full[x], NT == 2 ? np & 1 : (np >> 1) & 1);
+        const int x = C::buffer(np);
+        const uint32_t s_addr = tmem + lanes + C::score_col(t, x);
+        const int key0 = tile_key(u, j);
+        wait(&s_full[t][x], C::parity(np));
         tc_after();
         float s[KT];
 #pragma unroll
         for (int c = 0; c < KT / 32; c++) tmem_ld32(s_addr + c * 32, s + c * 32);
         tmem_wait_ld();
-        const int key0 = tile_key(u, j), hm = held[np % kHeldRing];
-        if (!open_tile(u, key0) || hm != kAll) {
+        const int hm = held[np % kHeldRing];
+        if (key0 > open_to || (key0 < open_from && key0 >= open_sinks) || hm != kAll) {
           // the row's keys of this tile: below its position and the sequence's
           // end, inside the window or among the sinks, on a page that exists
           const int end = min(p + 1, u.hi) - key0;
@@ -585,66 +593,84 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
                            bit_range(0, min(end, min(A.sinks, 1 << 30) - key0) - 32 * w);
             if (!(hm >> (2 * w) & 1)) see &= 0xFFFF0000u;
             if (!(hm >> (2 * w + 1) & 1)) see &= 0xFFFFu;
+            if (see != 0xFFFFFFFFu) {  // (a border cuts few of a warp's words)
 #pragma unroll
-            for (int c = 0; c < 32; c++)
-              if (!(see >> c & 1)) s[32 * w + c] = -INFINITY;
-          }
-        }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int c = 4; c < KT; c += 8) {
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            mx[e] = c + 4 + e < KT ? max3(mx[e], s[c + e], s[c + 4 + e]) : fmaxf(mx[e], s[c + e]);
-        }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
-        const bool grow = top > ref + 8.0f || (ref == -INFINITY && top > -INFINITY);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float f = grow ? (ref == -INFINITY ? 0.0f : ex2(ref - top)) : 1.0f;
-          if (grow) {
-            ref = top;
-            l *= f;
-          }
-          if (j > 0) {
-            // O holds the tiles before this one: with two row tiles the commit
-            // of these scores covers them, with one it does not
-            if constexpr (NT == 1) wait(&pv_done, (np - 1) & 1);
-            tc_after();
-#pragma unroll 1
-            for (int c = 0; c < Dh / 32; c++) {
-              float o[32];
-              tmem_ld32(o_addr + c * 32, o);
-              tmem_wait_ld();
-              uint32_t r[32];
-#pragma unroll
-              for (int e = 0; e < 32; e++) r[e] = __float_as_uint(o[e] * f);
-              tmem_st32(o_addr + c * 32, r);
+              for (int c = 0; c < 32; c++)
+                if (!(see >> c & 1)) s[32 * w + c] = -INFINITY;
             }
           }
         }
-        const float sub = ref == -INFINITY ? 0.0f : ref;
-        const uint64_t scale2 = pair(kLog2e, kLog2e), sub2 = pair(-sub, -sub);
-        uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int c = 0; c < KT / 64; c++) {
+        for (int part = 0; part < C::NH; part++) {
+          const float *sp = s + 64 * part;
+          // P = 2^(s log2 e - ref) of 64 keys, packed; their share of the sum
           uint32_t r[32];
+          auto exps = [&]() {
+            const float sub = ref == -INFINITY ? 0.0f : ref;
+            const uint64_t scale2 = pair(kLog2e, kLog2e), sub2 = pair(-sub, -sub);
+            uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int e = 0; e < 32; e++) {
-            const float2 v = unpair(fma2(pair(s[c * 64 + 2 * e], s[c * 64 + 2 * e + 1]), scale2, sub2));
-            const float a = ex2(v.x), b = ex2(v.y);
-            sum[e & 3] = add2(sum[e & 3], pair(a, b));
-            r[e] = pack2<T>(a, b);
+            for (int e = 0; e < 32; e++) {
+              float2 v = unpair(fma2(pair(sp[2 * e], sp[2 * e + 1]), scale2, sub2));
+              v = make_float2(ex2(v.x), ex2(v.y));
+              sum[e & 3] = add2(sum[e & 3], pair(v.x, v.y));
+              r[e] = pack2<T>(v.x, v.y);
+            }
+            const float2 v = unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+            return v.x + v.y;
+          };
+          // The reference of the keys before nearly always still holds, so P is
+          // made with it and its sum tells: at most 2^8 means that no P is
+          // larger. (No maximum is taken on this path: P of 64 keys sums to 64 at
+          // most where the reference is the true maximum.)
+          float sum = 0.0f;
+          bool holds = false;
+          if (j > 0 || part > 0) {
+            sum = exps();
+            holds = sum <= 256.0f;
+            if (ref == -INFINITY) {  // nothing seen so far: still so? (rows of nobody: always)
+              float top = -INFINITY;
+              if (p >= 0) {
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) top = max3(top, sp[c], sp[c + 1]);
+              }
+              holds = !(top > -INFINITY) && (p < 0 || !isnan(sum));
+            }
           }
-          tmem_st32(s_addr + c * 32, r);
+          if (!__all_sync(0xffffffffu, holds)) {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], sp[c], sp[c + 1]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
+            const bool grow = top > ref;
+            const float f = grow && ref > -INFINITY ? ex2(ref - top) : grow ? 0.0f : 1.0f;
+            if (grow) ref = top;
+            l *= f;
+            if (j > 0 || part > 0) {
+              // O must hold all keys before these: the scores' commit says so
+              // for the tile before (with one score buffer), pv_done else
+              if (C::NB == 2 || part > 0) wait(&pv_done[t], (C::NB == 2 ? np - 1 : np) & 1);
+              tc_after();
+#pragma unroll 1
+              for (int c = 0; c < Dh / 16; c++) {
+                float o[16];
+                tmem_ld16(o_addr + c * 16, o);
+                tmem_wait_ld();
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) w[e] = __float_as_uint(o[e] * f);
+                tmem_st16(o_addr + c * 16, w);
+              }
+            }
+            sum = exps();
+          }
+          l += sum;
+          tmem_st32(s_addr + part * 32, r);
+          tmem_wait_st();
+          tc_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t][C::NH == 1 ? x : part]);
         }
-        {
-          const float2 v = unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-          l += v.x + v.y;
-        }
-        tmem_wait_st();
-        tc_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
       }
       // ---- the rows' results
       wait(&o_full[t], nu & 1);
@@ -660,9 +686,9 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
         if ((nodd[0] | nodd[1]) && valid) {
           // infinities and NaN of V that this row does see
           for (int k = 0; k < nodd[0] + nodd[1]; k++) {
-            const int half = k >= nodd[0];
-            const int key0 = tile_key(u, odd[nu % kOddRing][half][1 + k - (half ? nodd[0] : 0)]) + half * (KT / 2);
-            for (int key = key0; key < key0 + KT / 2; key++) {
+            const int h = k >= nodd[0];
+            const int k0 = tile_key(u, odd[nu % kOddRing][h][1 + k - (h ? nodd[0] : 0)]) + h * (KT / 2);
+            for (int key = k0; key < k0 + KT / 2; key++) {
               if (key >= u.hi || !sees_key(p, key, A.window, A.sinks)) continue;
               const int page = A.pt.table[(size_t)u.b * A.pt.max_pages + key / A.pt.page_size];
               if (page < 0 || page >= A.pt.num_pages) continue;
@@ -683,14 +709,14 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
           // a row that saw nothing: O may hold anything, its result is zeros
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            uint4 r = make_uint4(0, 0, 0, 0);
+            uint4 w = make_uint4(0, 0, 0, 0);
             if (ref > -INFINITY || isnan(l)) {
-              r.x = pack2<T>(o[8 * e] * inv, o[8 * e + 1] * inv);
-              r.y = pack2<T>(o[8 * e + 2] * inv, o[8 * e + 3] * inv);
-              r.z = pack2<T>(o[8 * e + 4] * inv, o[8 * e + 5] * inv);
-              r.w = pack2<T>(o[8 * e + 6] * inv, o[8 * e + 7] * inv);
+              w.x = pack2<T>(o[8 * e] * inv, o[8 * e + 1] * inv);
+              w.y = pack2<T>(o[8 * e + 2] * inv, o[8 * e + 3] * inv);
+              w.z = pack2<T>(o[8 * e + 4] * inv, o[8 * e + 5] * inv);
+              w.w = pack2<T>(o[8 * e + 6] * inv, o[8 * e + 7] * inv);
             }
-            *reinterpret_cast<uint4 *>(dst + c * 32 + 8 * e) = r;
+            *reinterpret_cast<uint4 *>(dst + c * 32 + 8 * e) = w;
           }
         }
       }
