@@ -160,9 +160,15 @@ int wg_spec_accept(wg_ctx *ctx, const int32_t *drafts, const int32_t *picks, int
  * (draft and drafts NULL) is plain sampling. -inf logits (filtered tokens)
  * have probability 0. The decisions are those of 64-bit arithmetic. A row
  * with NaN, +inf or nothing but -inf yields some valid token and is reported
- * by wg_sync. k <= 32, V <= 2^21, temperature in [1e-4, 1e4]. */
+ * by wg_sync. k <= 32, V <= 2^21, (2k + 1) batch <= 65535, temperature in
+ * [1e-4, 1e4]. `workspace` (8-byte aligned device memory of at least
+ * wg_spec_sample_workspace bytes, any content): calls that may overlap on the
+ * GPU need one each. */
 int wg_spec_sample(wg_ctx *ctx, const float *target, const float *draft, const int32_t *drafts, int batch, int k,
-                   int V, double temperature, const float *u, int32_t *picks);
+                   int V, double temperature, const float *u, int32_t *picks, void *workspace,
+                   size_t workspace_bytes);
+/* The workspace of a wg_spec_sample of this shape. */
+int wg_spec_sample_workspace(wg_ctx *ctx, int batch, int k, int V, size_t *bytes);
 
 /* counters[0..n) += delta on the device (advances the positions of a
  * replayed decode step). */

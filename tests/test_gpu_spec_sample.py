@@ -209,9 +209,15 @@ def test_refusals():
         with pytest.raises(A):
             spec_sample(t, d, drafts, u, temperature=T)
     c, L = wg.context(), _lib.lib()
-    x = t.data_ptr()
-    assert L.wg_spec_sample(c.handle, x, x, x, 1, 33, 8, 1.0, x, x) == _lib.WG_INVALID_SHAPE
-    assert L.wg_spec_sample(c.handle, x, x, x, 1, 1, 0, 1.0, x, x) == _lib.WG_INVALID_SHAPE
-    assert L.wg_spec_sample(c.handle, x, None, x, 1, 1, 8, 1.0, x, x) == _lib.WG_INVALID_ARGUMENT
-    assert L.wg_spec_sample(c.handle, x + 2, x, x, 1, 1, 8, 1.0, x, x) == _lib.WG_INVALID_ARGUMENT
-    assert L.wg_spec_sample(c.handle, None, None, None, 0, 0, 8, 1.0, None, None) == 0
+    x, n = t.data_ptr(), ctypes.c_size_t()
+
+    def call(target=x, draft=x, drafts=x, batch=1, k=1, V=8, ws=x, ws_bytes=1 << 20):
+        return L.wg_spec_sample(c.handle, target, draft, drafts, batch, k, V, 1.0, x, x, ws, ws_bytes)
+
+    I, A, U = _lib.WG_INVALID_SHAPE, _lib.WG_INVALID_ARGUMENT, _lib.WG_UNSUPPORTED
+    for st, kw in [(I, dict(k=33)), (I, dict(k=-1)), (I, dict(V=0)), (I, dict(V=(1 << 21) + 1)), (I, dict(batch=-1)),
+                   (U, dict(batch=30000)), (A, dict(draft=None)), (A, dict(drafts=None)), (A, dict(target=x + 2)),
+                   (A, dict(ws=None)), (A, dict(ws=x + 4)), (A, dict(ws_bytes=23)), (0, dict(batch=0))]:
+        assert call(**kw) == st, kw
+    assert L.wg_spec_sample_workspace(c.handle, 1, 1, 8, ctypes.byref(n)) == 0 and n.value == 24
+    assert L.wg_spec_sample_workspace(c.handle, 1, 40, 8, ctypes.byref(n)) == I

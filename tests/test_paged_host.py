@@ -25,7 +25,7 @@ def test_c_entry_points_reject_a_null_context():
     assert L.wg_paged_rope_kv(None, None, 1, 1, None, 1, 1, 64, None, 1e4, None, None, 1e-5, None, ctypes.byref(kv)) \
         == _lib.WG_INVALID_ARGUMENT
     assert L.wg_paged_attention_workspace(None, 64, ctypes.byref(ctypes.c_size_t())) == _lib.WG_INVALID_ARGUMENT
-    assert L.wg_spec_sample(None, None, None, None, 1, 0, 8, 1.0, None, None) == _lib.WG_INVALID_ARGUMENT
+    assert L.wg_spec_sample(None, None, None, None, 1, 0, 8, 1.0, None, None, None, 0) == _lib.WG_INVALID_ARGUMENT
 
 
 def test_host_tensors_are_refused():

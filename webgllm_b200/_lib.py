@@ -96,7 +96,8 @@ SIGNATURES = {
     "wg_argmax": (_I, [_P, _P, _I, _I, _P]),
     "wg_add_i32": (_I, [_P, _P, _I, _I]),
     "wg_spec_accept": (_I, [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P]),
-    "wg_spec_sample": (_I, [_P, _P, _P, _P, _I, _I, _I, ctypes.c_double, _P, _P]),
+    "wg_spec_sample": (_I, [_P, _P, _P, _P, _I, _I, _I, ctypes.c_double, _P, _P, _P, _SZ]),
+    "wg_spec_sample_workspace": (_I, [_P, _I, _I, _I, ctypes.POINTER(_SZ)]),
     # include/webgllm_paged.h
     "wg_paged_rope_kv": (_I, [_P, _P, _I, _I, _P, _I, _I, _I, _P, ctypes.c_double, _P, _P, ctypes.c_float, _P, _P]),
     "wg_paged_attention": (_I, [_P, _P, _I, _I, _P, _I, _I, _I, _P, _P, _I, _I, _P, _P, _SZ]),

@@ -255,25 +255,44 @@ int wg_spec_accept(wg_ctx *ctx, const int32_t *drafts, const int32_t *picks, int
                 "wg_spec_accept");
 }
 
-int wg_spec_sample(wg_ctx *ctx, const float *target, const float *draft, const int32_t *drafts, int batch, int k,
-                   int V, double temperature, const float *u, int32_t *picks) {
-  WG_BEGIN(ctx);
+static int check_sample(wg_ctx *ctx, const char *what, int batch, int k, int V) {
   if (batch < 0 || k < 0 || k > wg::kSampleMaxDrafts || V < 1 || V > wg::kSampleMaxVocab)
-    return dfail(ctx, WG_INVALID_SHAPE, "wg_spec_sample: batch %d, k %d (<= %d), V %d (<= %d)", batch, k,
+    return dfail(ctx, WG_INVALID_SHAPE, "%s: batch %d, k %d (<= %d), V %d (<= %d)", what, batch, k,
                  wg::kSampleMaxDrafts, V, wg::kSampleMaxVocab);
-  if (batch > (1 << 24)) return dfail(ctx, WG_UNSUPPORTED, "wg_spec_sample: batch %d", batch);
+  if ((long long)batch * (2 * k + 1) > 65535)
+    return dfail(ctx, WG_UNSUPPORTED, "%s: %d sequences of %d rows in one call", what, batch, 2 * k + 1);
+  return WG_OK;
+}
+
+int wg_spec_sample(wg_ctx *ctx, const float *target, const float *draft, const int32_t *drafts, int batch, int k,
+                   int V, double temperature, const float *u, int32_t *picks, void *workspace,
+                   size_t workspace_bytes) {
+  WG_BEGIN(ctx);
+  if (int st = check_sample(ctx, "wg_spec_sample", batch, k, V)) return st;
   if (!(temperature >= 1e-4 && temperature <= 1e4))
     return dfail(ctx, WG_INVALID_ARGUMENT, "wg_spec_sample: temperature %g outside [1e-4, 1e4]", temperature);
   if (!batch) return WG_OK;
-  if (!target || !u || !picks || (k && (!draft || !drafts)))
+  if (!target || !u || !picks || !workspace || (k && (!draft || !drafts)))
     return dfail(ctx, WG_INVALID_ARGUMENT, "wg_spec_sample: null");
   for (const void *p : {(const void *)target, (const void *)draft, (const void *)drafts, (const void *)u,
                         (const void *)picks})
     if ((uintptr_t)p & 3u) return dfail(ctx, WG_INVALID_ARGUMENT, "wg_spec_sample: misaligned tensor");
+  const size_t need = wg::spec_sample_workspace(batch, k, V);
+  if (((uintptr_t)workspace & 7u) || workspace_bytes < need)
+    return dfail(ctx, WG_INVALID_ARGUMENT, "wg_spec_sample: a workspace of %zu bytes, %zu needed (8-byte aligned)",
+                 workspace_bytes, need);
   return finish(ctx,
-                wg::launch_spec_sample(target, draft, drafts, batch, k, V, temperature, u, picks, ctx->d_flags,
-                                       ctx->stream, ctx->pdl),
+                wg::launch_spec_sample(target, draft, drafts, batch, k, V, temperature, u, picks, workspace,
+                                       ctx->d_flags, ctx->stream, ctx->pdl),
                 "wg_spec_sample");
+}
+
+int wg_spec_sample_workspace(wg_ctx *ctx, int batch, int k, int V, size_t *bytes) {
+  if (!ctx || !bytes) return WG_INVALID_ARGUMENT;
+  *bytes = 0;
+  if (int st = check_sample(ctx, "wg_spec_sample_workspace", batch, k, V)) return st;
+  *bytes = wg::spec_sample_workspace(batch, k, V);
+  return WG_OK;
 }
 
 int wg_add_i32(wg_ctx *ctx, int32_t *counters, int n, int delta) {

@@ -67,8 +67,9 @@ cudaError_t launch_spec_accept(const int32_t *drafts, const int32_t *picks, int 
                                int32_t *out_len, int32_t *accepted, cudaStream_t s, bool pdl);
 // spec_sample.cu
 constexpr int kSampleMaxDrafts = 32, kSampleMaxVocab = 1 << 21;
+size_t spec_sample_workspace(int batch, int k, int V);
 cudaError_t launch_spec_sample(const float *target, const float *draft, const int32_t *drafts, int batch, int k, int V,
-                               double temperature, const float *u, int32_t *picks, unsigned *flags, cudaStream_t s,
-                               bool pdl);
+                               double temperature, const float *u, int32_t *picks, void *workspace, unsigned *flags,
+                               cudaStream_t s, bool pdl);
 
 }  // namespace wg

@@ -124,6 +124,15 @@ __device__ __forceinline__ void trace_record(unsigned long long *buf, unsigned l
   r[7] = ((unsigned long long)launch << 32) | cta;
 }
 
+// ---- exponentials ----------------------------------------------------------
+
+// 2^x, results below 2^-126 as 0 (one instruction; good to 2^-22 relative).
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // ---- fp16 helpers ----------------------------------------------------------
 
 // (a & b) | c

@@ -47,13 +47,6 @@ __device__ __forceinline__ bool nonfinite2(uint32_t u) {
   return (u & e) == e || (u >> 16 & e) == e;
 }
 
-// 2^x, results below 2^-126 as 0 (one instruction; good to 2^-22 relative).
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // Rows of sequence b: [r0, r0 + n), clamped to the buffers.
 __device__ __forceinline__ void seq_rows(const PagedRows &a, int b, int &r0, int &n) {
   if (a.row_start) {

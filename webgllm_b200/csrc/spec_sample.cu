@@ -7,10 +7,16 @@
 //   from p_k. Together the kept tokens and the drawn one are distributed as
 //   samples of the target.
 //
-// A thread-block cluster serves a sequence: each CTA takes a slice of the
-// vocabulary of every row, and the CTAs exchange sums through distributed
-// shared memory, so one launch does everything and nothing is kept in global
-// memory.
+// Two launches. sample_stats_kernel streams every row once over the whole machine
+// (pieces of 8192 logits a CTA, all of its loads in flight at once) and leaves
+// (max, sum) of each piece in the workspace. spec_sample_kernel, a thread-block
+// cluster a sequence, (1) combines them, (2) decides acceptance, a lane a draft,
+// (3) makes the drawn row's weights in 64 bits, kept in shared memory where they
+// fit, a slice of the vocabulary a CTA, the CTAs' sums exchanged through
+// distributed shared memory, and (4) finds the token by the running sum over
+// CTAs, warps, lanes, and one lane's run. (In one launch, the clusters doing the
+// streaming too, 61 sequences of 11 rows of 65543 took 144 us: their phases run
+// in step, and the memory idles through the later ones.)
 // The answer is a whole number, so it must not hang on rounding. The
 // statistics that decide acceptance are fp32 exponentials (their sum is good
 // to kSlack), and a decision closer than that is taken again from sums of
@@ -18,7 +24,7 @@
 // throughout: p - q cancels where draft and target agree, and its running sum
 // is compared with u at a resolution of one token in V.
 // Bound: the (2k + 1) V logits of a sequence, read once (HBM), plus the 64-bit
-// exponentials of the drawn rows (2 V a sequence).
+// exponentials of the drawn rows (3 V a sequence, 12 operations each).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -34,13 +40,14 @@ namespace {
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleCluster = 16;  // largest cluster
+constexpr size_t kKeepBytes = 200 * 1024;  // of shared memory for the drawn rows' weights
 constexpr int kMaxRows = 2 * kSampleMaxDrafts + 1;
 // Relative error bound of u q(d) / p(d) when the two normalising sums come from
 // fp32 exponentials. A term exp(-a) is off by at most a 2^-22 + 2^-21 of
-// itself, and terms that matter have a <= ln V (15 at the largest vocabulary);
-// a thread adds at most V / (16 x 512) = 256 of them, each addition off by at
-// most 2^-24. Both sums: below 2 (4e-6 + 1.6e-5) = 4e-5.
-constexpr double kSlack = 4e-5;
+// itself, and terms that matter have a <= ln V (15 at the largest vocabulary):
+// 4e-6; a thread adds 36 of them and the CTA's threads 13 levels deep, each
+// addition off by at most 2^-24: 3e-6. Both sums: below 2e-5.
+constexpr double kSlack = 2e-5;
 
 struct SampleArgs {
   const float *target;    // [k + 1][batch][V]
@@ -49,20 +56,13 @@ struct SampleArgs {
   const float *u;         // [batch][k + 1]
   int32_t *picks;         // [k + 1][batch]
   int batch, k, V;
+  float2 *stats;          // [2k + 1][batch][chunks]: (max, sum) of a row's pieces
+  int chunks;
   int slice;              // vocabulary entries per CTA
+  int keep;               // arrays of the slice's weights kept in shared memory: p's, then q's
   double temperature;
   unsigned *flags;
 };
-
-struct MaxSum {
-  float m, s;
-};
-
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return MaxSum{m, 0.0f};
-  return MaxSum{m, a.s * exp2f((a.m - m) * c) + b.s * exp2f((b.m - m) * c)};
-}
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
@@ -70,56 +70,139 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   return v;
 }
 
-// The sum of one double per thread over the whole cluster, the same bits in
-// every thread of every CTA (summed in rank order).
-struct ClusterSum {
-  double warp[kSampleWarps];
-  double cta;
-};
+// Running sum of the 16 lanes' values (lanes 16 .. 31 as 0 .. 15), inclusive.
+__device__ __forceinline__ double scan16(double v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, v, o, 16);
+    if ((lane & 15) >= o) v += t;
+  }
+  return v;
+}
 
-__device__ double cta_sum(double v, ClusterSum &sh) {
+__device__ __forceinline__ double last16(double scanned) { return __shfl_sync(0xffffffffu, scanned, 15); }
+
+// The sum of one double per thread over the CTA, the same bits in every thread;
+// `warp_part` afterwards holds the warps' sums.
+__device__ __forceinline__ double cta_sum(double v, double *warp_part) {
   v = warp_sum_f64(v);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = v;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) warp_part[threadIdx.x >> 5] = v;
   __syncthreads();
-  double t = 0.0;
-#pragma unroll
-  for (int i = 0; i < kSampleWarps; i++) t += sh.warp[i];
-  return t;
+  return last16(scan16(warp_part[lane & 15], lane));
 }
 
-__device__ double cluster_sum(double v, ClusterSum &sh, double *before = nullptr, double *own = nullptr) {
-  cg::cluster_group cl = cg::this_cluster();
-  const double mine = cta_sum(v, sh);
-  if (threadIdx.x == 0) sh.cta = mine;
-  if (own) *own = mine;
-  cl.sync();
-  double t = 0.0;
-  const int me = (int)cl.block_rank(), n = (int)cl.num_blocks();
-  for (int i = 0; i < n; i++) {
-    if (before && i == me) *before = t;
-    t += *cl.map_shared_rank(&sh.cta, i);
+// The running sums of the cluster's CTAs (their *mine), the same bits in every
+// CTA: rank i's share is [incl(i - 1), incl(i)). Needs a cluster barrier
+// between the writes and the call.
+__device__ __forceinline__ double ranks_scan(const double *mine, int lane, int CL) {
+  const int i = lane & 15;
+  return scan16(i < CL ? *cg::this_cluster().map_shared_rank(mine, i) : 0.0, lane);
+}
+// exp((x - max) / T) in 64 bits, off by less than 2^-50: 2^(n / 16) from a
+// table (16 doubles in shared memory: one bank row, no conflicts whatever the
+// lanes pick), n the nearest to 16 log2 e (x - max) / T, times the Taylor
+// polynomial of the rest (at most ln 2 / 32 away: degree 7 leaves 2e-18).
+// Below 2^-1000: 0.
+__constant__ double kRoots[16] = {
+    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
+    1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
+    1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+    1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+struct Exp64 {
+  double scale, shift;  // 16 log2 e / T, and - max times it
+  const double *table;
+  __device__ __forceinline__ double operator()(float x) const {
+    const double y = fma((double)x, scale, shift);
+    if (!(y > -16000.0)) return 0.0;
+    const double t = y + 6755399441055744.0;  // n in the low bits
+    const int n = __double2loint(t);
+    const double f = y - (t - 6755399441055744.0);
+    constexpr double h = 0.04332169878499658;  // ln 2 / 16
+    constexpr double h2 = h * h, h3 = h2 * h, h4 = h2 * h2;
+    double p = h4 * h3 / 5040.0;
+    p = fma(p, f, h3 * h3 / 720.0);
+    p = fma(p, f, h3 * h2 / 120.0);
+    p = fma(p, f, h4 / 24.0);
+    p = fma(p, f, h3 / 6.0);
+    p = fma(p, f, h2 / 2.0);
+    p = fma(p, f, h);
+    p = fma(p, f, 1.0);
+    const double r = p * table[n & 15];
+    return __hiloint2double(__double2hiint(r) + ((n >> 4) << 20), __double2loint(r));
   }
-  cl.sync();  // sh.cta may be written again
-  return t;
-}
+};
 
-__global__ void __launch_bounds__(kSampleThreads) spec_sample_kernel(const SampleArgs a) {
+constexpr int kChunk = 8192;        // logits of a piece
+constexpr int kStatsThreads = 256;  // 8 float4 a thread, and the row's unaligned ends
+
+// (max, sum of exp((x - max) / T)) of piece blockIdx.x of row blockIdx.y (rows in
+// memory order: the target's, then the draft's).
+__global__ void __launch_bounds__(kStatsThreads) sample_stats_kernel(const SampleArgs a) {
   pdl_trigger();
   pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, V = a.V;
+  const int rows_t = (a.k + 1) * a.batch, r = blockIdx.y;
+  const float *p = r < rows_t ? a.target + (size_t)r * V : a.draft + (size_t)(r - rows_t) * V;
+  const float c = (float)(1.4426950408889634 / a.temperature);
+  // the piece's aligned float4s; the row's ends (fewer than 4 logits each) go to
+  // its first and its last piece
+  const int lead = min((int)((4 - ((uintptr_t)p >> 2 & 3)) & 3), V), quads = (V - lead) / 4;
+  const int q0 = blockIdx.x * (kChunk / 4);
+  const float4 *x = reinterpret_cast<const float4 *>(p + lead);
+  float4 v[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const int i = q0 + tid + e * kStatsThreads;
+    v[e] = i < quads ? __ldg(x + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  }
+  float end = -INFINITY;
+  const int tail = lead + 4 * quads + tid - 4;
+  if (blockIdx.x == 0 && tid < lead) end = p[tid];
+  if (blockIdx.x == gridDim.x - 1 && tid >= 4 && tail < V) end = p[tail];
+  float m = end;
+#pragma unroll
+  for (int e = 0; e < 8; e++) m = fmaxf(fmaxf(m, fmaxf(v[e].x, v[e].y)), fmaxf(v[e].z, v[e].w));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  __shared__ float sm[kStatsThreads / 32], ss[kStatsThreads / 32];
+  if (lane == 0) sm[tid >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kStatsThreads / 32; i++) m = fmaxf(m, sm[i]);
+  const float sub = m > -INFINITY ? m : 0.0f;  // (-inf throughout: every term 0; NaN: NaN)
+  float s = ex2((end - sub) * c);
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+    s += (ex2((v[e].x - sub) * c) + ex2((v[e].y - sub) * c)) + (ex2((v[e].z - sub) * c) + ex2((v[e].w - sub) * c));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) ss[tid >> 5] = s;
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int i = 1; i < kStatsThreads / 32; i++) s += ss[i];
+    a.stats[(size_t)r * a.chunks + blockIdx.x] = make_float2(m, s);
+  }
+}
+
+__global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const SampleArgs a) {
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), CL = (int)cl.num_blocks();
   const int b = blockIdx.x / CL;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int k = a.k, R = 2 * k + 1, V = a.V;
-  const int v0 = min((long long)V, (long long)rank * a.slice), v1 = min((long long)V, (long long)v0 + a.slice);
-  __shared__ MaxSum warp_ms[kMaxRows][kSampleWarps];
-  __shared__ MaxSum cta_ms[kMaxRows];
+  extern __shared__ __align__(16) double kept[];  // [keep][slice] weights of the drawn row
   __shared__ float row_m[kMaxRows];
   __shared__ double row_z[kMaxRows];
-  __shared__ ClusterSum csum;
-  __shared__ double groups[kSampleWarps];
-  __shared__ int found;
+  __shared__ double table[16], warp_part[kSampleWarps], cta_part[4];
+  __shared__ int s_n, s_owner;
+  static_assert(kSampleWarps == 16 && kSampleCluster == 16, "16 lanes scan");
+
+  pdl_trigger();
+  if (tid < 16) table[tid] = kRoots[tid];
+  pdl_wait();
 
   // rows 0 .. k: the target's; k + 1 .. 2k: the draft's
   auto row = [&](int r) {
@@ -127,90 +210,105 @@ __global__ void __launch_bounds__(kSampleThreads) spec_sample_kernel(const Sampl
   };
   const float c = (float)(1.4426950408889634 / a.temperature);
 
-  // ---- maximum and sum of every row
-  for (int r = 0; r < R; r++) {
-    const float *x = row(r);
-    MaxSum ms{-INFINITY, 0.0f};
-    auto one = [&](float v) {
-      if (v > ms.m) {
-        ms.s *= exp2f((ms.m - v) * c);
-        ms.m = v;
-      }
-      if (ms.m > -INFINITY) ms.s += exp2f((v - ms.m) * c);
-    };
-    // the 16-byte aligned middle of the slice four at a time
-    const int lead = min((int)((4 - (((uintptr_t)(x + v0) >> 2) & 3)) & 3), v1 - v0);
-    const int quads = (v1 - v0 - lead) / 4;
-    if (tid < lead) one(x[v0 + tid]);
-    const float4 *x4 = reinterpret_cast<const float4 *>(x + v0 + lead);
-#pragma unroll 4
-    for (int i = tid; i < quads; i += kSampleThreads) {
-      const float4 v = x4[i];
-      const float m = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-      if (m > ms.m) {
-        ms.s *= exp2f((ms.m - m) * c);
-        ms.m = m;
-      }
-      if (ms.m > -INFINITY)
-        ms.s += (exp2f((v.x - ms.m) * c) + exp2f((v.y - ms.m) * c)) +
-                (exp2f((v.z - ms.m) * c) + exp2f((v.w - ms.m) * c));
+  // ---- (1) every row's maximum and sum, from its pieces'; meanwhile the last
+  // warp fetches what acceptance needs (lane j: draft j)
+  int d = -1;
+  float xp_d = 0.0f, xq_d = 0.0f;
+  double u_d = 0.0;
+  if (warp == kSampleWarps - 1 && lane < k) {
+    d = a.drafts[(size_t)b * k + lane];
+    u_d = (double)a.u[(size_t)b * (k + 1) + lane];
+    if (u_d >= 1.0) u_d = 1.0 - 0x1p-24;
+    if (d >= 0 && d < V) {
+      xp_d = row(lane)[d];
+      xq_d = row(k + 1 + lane)[d];
     }
-    const int tail = v0 + lead + 4 * quads + tid;
-    if (tail < v1) one(x[tail]);
+  }
+  for (int r = warp; r < R; r += kSampleWarps) {
+    const float2 *st = a.stats + ((size_t)r * a.batch + b) * a.chunks;
+    float2 v = lane < a.chunks ? __ldcg(st + lane) : make_float2(-INFINITY, 0.0f);
+    float m = v.x;
+    for (int i = lane + 32; i < a.chunks; i += 32) m = fmaxf(m, __ldcg(st + i).x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      ms = join(ms, MaxSum{__shfl_xor_sync(0xffffffffu, ms.m, o), __shfl_xor_sync(0xffffffffu, ms.s, o)}, c);
-    if (lane == 0) warp_ms[r][warp] = ms;
-  }
-  __syncthreads();
-  for (int r = tid; r < R; r += kSampleThreads) {
-    MaxSum ms = warp_ms[r][0];
-    for (int i = 1; i < kSampleWarps; i++) ms = join(ms, warp_ms[r][i], c);
-    cta_ms[r] = ms;
-  }
-  cl.sync();
-  for (int r = tid; r < R; r += kSampleThreads) {
-    float m = -INFINITY;
-    for (int i = 0; i < CL; i++) m = fmaxf(m, cl.map_shared_rank(&cta_ms[r], i)->m);
-    double z = 0.0;
-    for (int i = 0; i < CL; i++) {
-      const MaxSum ms = *cl.map_shared_rank(&cta_ms[r], i);
-      if (ms.m > -INFINITY) z += (double)ms.s * (double)exp2f((ms.m - m) * c);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    // (a piece of nothing: -inf and 0, or a NaN on its way)
+    auto share = [&](float2 w) { return (double)w.y * (w.x > -INFINITY ? (double)ex2((w.x - m) * c) : 1.0); };
+    double z = share(v);
+    for (int i = lane + 32; i < a.chunks; i += 32) z += share(__ldcg(st + i));
+    z = warp_sum_f64(z);
+    if (lane == 0) {
+      row_m[r] = m;
+      row_z[r] = z;
     }
-    row_m[r] = m;
-    row_z[r] = z;
   }
   __syncthreads();
-  // (a peer's cta_ms is not written again: no barrier is owed for it until exit)
 
-  // exp((x - max) / T) in 64 bits
-  auto weight = [&](float x, float m) { return exp(((double)x - (double)m) / a.temperature); };
+  const int v0 = (int)min((long long)V, (long long)rank * a.slice), n_v = (int)min((long long)a.slice, (long long)V - v0);
+  // this warp's run of the slice; each lane a run of it, of odd length (the
+  // lanes then meet no bank conflicts)
+  const int per_lane = (n_v + kSampleThreads - 1) / kSampleThreads | 1;
+  const int w0 = min(n_v, warp * 32 * per_lane), w1 = min(n_v, w0 + 32 * per_lane);
+  const int l0 = min(w1, w0 + lane * per_lane), l1 = min(w1, l0 + per_lane);
+  const double scale = 16.0 * 1.4426950408889634074 / a.temperature;
+  auto weights = [&](int r) { return Exp64{scale, -(double)row_m[r] * scale, table}; };
+  // f(i, logit) over this warp's run of a row, eight loads a lane in flight
+  auto each = [&](const float *x, auto &&f) {
+    for (int i0 = w0 + lane; i0 < w1; i0 += 256) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = i0 + 32 * e < w1 ? __ldg(x + i0 + 32 * e) : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (i0 + 32 * e < w1) f(i0 + 32 * e, v[e]);
+    }
+  };
+  // the sum of row r's weights over the whole vocabulary
   auto exact_sum = [&](int r) {
-    const float *x = row(r);
-    const float m = row_m[r];
+    const Exp64 w = weights(r);
     double s = 0.0;
-    for (int i = v0 + tid; i < v1; i += kSampleThreads) s += weight(x[i], m);
-    return cluster_sum(s, csum);
+    each(row(r) + v0, [&](int, float x) { s += w(x); });
+    s = cta_sum(s, warp_part);
+    if (tid == 0) cta_part[0] = s;
+    cl.sync();
+    s = last16(ranks_scan(&cta_part[0], lane, CL));
+    cl.sync();  // cta_part may be written again
+    return s;
   };
 
-  // ---- acceptance: the same in every thread of the cluster
+  // ---- (2) acceptance: lane j decides draft j, the same in every CTA
   int n = 0;
-  for (; n < k; n++) {
-    const int d = a.drafts[(size_t)b * k + n];
-    double u = (double)a.u[(size_t)b * (k + 1) + n];
-    if (u >= 1.0) u = 1.0 - 0x1p-24;
-    double pe = 0.0, qe = 0.0;
-    if (d >= 0 && d < V) {
-      pe = weight(row(n)[d], row_m[n]);
-      qe = weight(row(k + 1 + n)[d], row_m[k + 1 + n]);
+  if (k > 0) {
+    if (warp == kSampleWarps - 1) {
+      bool kept_it = false, close = false;
+      if (lane < k && d >= 0 && d < V) {
+        const double lhs = u_d * weights(k + 1 + lane)(xq_d) * row_z[lane];
+        const double rhs = weights(lane)(xp_d) * row_z[k + 1 + lane];
+        kept_it = lhs < rhs;
+        close = fabs(lhs - rhs) <= kSlack * rhs && rhs > 0.0;
+      }
+      const unsigned stop = __ballot_sync(0xffffffffu, lane < k && (!kept_it || close));
+      const unsigned near_ = __ballot_sync(0xffffffffu, close);
+      // the first that is not clearly kept; negative: too close for the fp32 sums
+      const int first = stop ? __ffs(stop) - 1 : k;
+      if (lane == 0) s_n = first < k && (near_ >> first & 1) ? -1 - first : first;
     }
-    double lhs = u * (qe / row_z[k + 1 + n]), rhs = pe / row_z[n];
-    if (fabs(lhs - rhs) <= kSlack * rhs && rhs > 0.0) {
-      const double zq = exact_sum(k + 1 + n), zp = exact_sum(n);
-      lhs = u * (qe / zq);
-      rhs = pe / zp;
-    }
-    if (!(lhs < rhs)) break;
+    __syncthreads();
+    n = s_n;
+    if (n < 0)  // from there on one by one
+      for (n = -1 - n; n < k; n++) {
+        const int dd = a.drafts[(size_t)b * k + n];
+        double u = (double)a.u[(size_t)b * (k + 1) + n];
+        if (u >= 1.0) u = 1.0 - 0x1p-24;
+        if (dd < 0 || dd >= V) break;
+        const double pe = weights(n)(row(n)[dd]), qe = weights(k + 1 + n)(row(k + 1 + n)[dd]);
+        const double lhs = u * qe * row_z[n], rhs = pe * row_z[k + 1 + n];
+        if (fabs(lhs - rhs) <= kSlack * rhs && rhs > 0.0) {
+          const double zq = exact_sum(k + 1 + n), zp = exact_sum(n);
+          if (!(u * (qe / zq) < pe / zp)) break;
+        } else if (!(lhs < rhs)) {
+          break;
+        }
+      }
   }
 
   // rows without probabilities (NaN, +inf, -inf throughout): a token all the
@@ -233,105 +331,163 @@ __global__ void __launch_bounds__(kSampleThreads) spec_sample_kernel(const Sampl
     return;
   }
 
-  // ---- the draw: from max(p - q, 0) of row n, or from p of row k
-  const float *xp = row(n), *xq = n < k ? row(k + 1 + n) : nullptr;
-  const float mp = row_m[n], mq = n < k ? row_m[k + 1 + n] : 0.0f;
+  // ---- (3) the weights of the draw: of max(p - q, 0) of row n, or of p of row k
+  const bool diff = n < k;
+  const float *xp = row(n) + v0, *xq = diff ? row(k + 1 + n) + v0 : nullptr;
+  const Exp64 wp = weights(n), wq = weights(diff ? k + 1 + n : n);
   double ip = 1.0, iq = 0.0;
-  if (n < k) {
-    ip = 1.0 / exact_sum(n);
-    iq = 1.0 / exact_sum(k + 1 + n);
+  double *const kept_q = kept + a.slice;
+  if (diff) {
+    double sp = 0.0, sq = 0.0;
+    each(xq, [&](int i, float x) {
+      const double e = wq(x);
+      if (a.keep == 2) kept_q[i] = e;
+      sq += e;
+    });
+    each(xp, [&](int i, float x) {
+      const double e = wp(x);
+      if (a.keep) kept[i] = e;
+      sp += e;
+    });
+    sp = cta_sum(sp, warp_part);
+    sq = cta_sum(sq, warp_part);
+    if (tid == 0) {
+      cta_part[1] = sp;
+      cta_part[2] = sq;
+    }
+    cl.sync();
+    const double rp = ranks_scan(&cta_part[1], lane, CL), rq = ranks_scan(&cta_part[2], lane, CL);
+    ip = 1.0 / last16(rp);
+    iq = 1.0 / last16(rq);
+    // (where only p's weights fit, q's are made a second time)
+    if (a.keep == 1) each(xq, [&](int i, float x) { kept[i] = fmax(kept[i] * ip - wq(x) * iq, 0.0); });
+  } else if (a.keep) {
+    each(xp, [&](int i, float x) { kept[i] = wp(x); });
   }
-  int mode = n < k ? 0 : 1;  // 0: p - q; 1: p; 2: p without the rejected token
+  __syncwarp();
+  bool without = false;  // p without the rejected token instead
   auto mass = [&](int i) {
-    const double p = weight(xp[i], mp);
-    if (mode == 0) return fmax(p * ip - weight(xq[i], mq) * iq, 0.0);
-    return mode == 2 && i == dn ? 0.0 : fmax(p, 0.0);
+    if (without) return v0 + i == dn ? 0.0 : wp(xp[i]);
+    if (a.keep == 2) return diff ? fmax(kept[i] * ip - kept_q[i] * iq, 0.0) : kept[i];
+    if (a.keep == 1) return kept[i];
+    return diff ? fmax(wp(xp[i]) * ip - wq(xq[i]) * iq, 0.0) : wp(xp[i]);
   };
-  double total, before, mine;
+
+  // ---- (4) the token: the first whose running sum exceeds u times the total
+  double total, before, after, lane_sum, lane_head;
   for (;;) {
-    double s = 0.0;
-    for (int i = v0 + tid; i < v1; i += kSampleThreads) s += mass(i);
-    total = cluster_sum(s, csum, &before, &mine);
+    lane_sum = 0.0;
+    for (int i = l0; i < l1; i++) lane_sum += mass(i);
+    double s = lane_sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += t;
+    }
+    lane_head = __shfl_up_sync(0xffffffffu, s, 1);
+    if (lane == 0) lane_head = 0.0;
+    __syncthreads();
+    if (lane == 31) warp_part[warp] = s;
+    if (tid == 0) s_owner = -1;
+    __syncthreads();
+    const double warps = scan16(warp_part[lane & 15], lane);
+    if (warp > 0) lane_head += __shfl_sync(0xffffffffu, warps, warp - 1);
+    if (tid == 15) cta_part[3] = warps;
+    cl.sync();
+    const double ranks = ranks_scan(&cta_part[3], lane, CL);
+    total = last16(ranks);
+    after = __shfl_sync(0xffffffffu, ranks, rank);
+    before = __shfl_sync(0xffffffffu, ranks, rank ? rank - 1 : 0);
+    if (!rank) before = 0.0;
     // p and q may agree to the last bit everywhere: then the rejected token's
     // place goes to another token of p
-    if (mode != 0 || total > 0.0) break;
-    mode = 2;
+    if (!diff || without || total > 0.0) break;
+    without = true;
+    cl.sync();
   }
   double u = (double)a.u[(size_t)b * (k + 1) + k];
   if (!(u < 1.0)) u = 1.0 - 0x1p-24;
   if (!(u > 0.0)) u = 0.0;
-  const double goal = u * total;  // the token is the first whose running sum exceeds it
-  if (!(total > 0.0)) {  // all of p on a token that was rejected: q cannot have been a distribution
-    report();
-    return;
-  }
-  // the CTA whose slice holds the goal finds the token: runs of 512 entries,
-  // a running sum over warps and lanes
-  const bool owner = before <= goal && goal < before + mine;  // before + mine is the next CTA's before, to the bit
-  if (owner) {
-    double run = before;
-    int last = -1;  // the last entry with mass: where rounding left the goal behind the slice's sum
-    if (tid == 0) found = 0x7fffffff;
+  const double goal = u * total;
+  if (!(total > 0.0)) report();  // all of p on the rejected token: q was no distribution
+  // One CTA holds the goal. There the running sum at the head of every lane's
+  // run says which lane: the last one that has weight and whose head is not past
+  // the goal.
+  if (total > 0.0 && before <= goal && goal < after) {
+    double head = before + lane_head;
+    const unsigned here = __ballot_sync(0xffffffffu, lane_sum > 0.0 && head <= goal);
+    if (here && lane == 0) atomicMax(&s_owner, warp * 32 + 31 - __clz(here));
     __syncthreads();
-    for (int i0 = v0; i0 < v1; i0 += kSampleThreads) {
-      const int i = i0 + tid;
-      const double m = i < v1 ? mass(i) : 0.0;
-      if (m > 0.0) last = i;
-      double s = m;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
+    if (tid == s_owner) {
+      int pick = -1;
+      for (int i = l0; i < l1; i++) {
+        const double m = mass(i);
+        if (!(m > 0.0)) continue;
+        pick = i;  // (rounding may leave the goal past the run's own sum: its last weight then)
+        head += m;
+        if (head > goal) break;
       }
-      if (lane == 31) groups[warp] = s;
-      __syncthreads();
-      double head = run, all = 0.0;
-      for (int w = 0; w < kSampleWarps; w++) {
-        if (w < warp) head += groups[w];
-        all += groups[w];
-      }
-      if (m > 0.0 && head + s > goal) atomicMin(&found, i);
-      __syncthreads();
-      if (found != 0x7fffffff) break;
-      run += all;
+      a.picks[(size_t)n * a.batch + b] = v0 + pick;
     }
-    if (found == 0x7fffffff) {
-      __syncthreads();
-      if (tid == 0) found = -1;
-      __syncthreads();
-      if (last >= 0) atomicMax(&found, last);
-      __syncthreads();
-    }
-    if (tid == 0) a.picks[(size_t)n * a.batch + b] = found;
   }
+  cl.sync();  // peers may still read this CTA's shared memory
 }
 
 }  // namespace
 
+static int sample_chunks(int V) { return (V + kChunk - 1) / kChunk; }
+
+size_t spec_sample_workspace(int batch, int k, int V) {
+  return (size_t)batch * (2 * k + 1) * sample_chunks(V) * sizeof(float2);
+}
+
 cudaError_t launch_spec_sample(const float *target, const float *draft, const int32_t *drafts, int batch, int k, int V,
-                               double temperature, const float *u, int32_t *picks, unsigned *flags, cudaStream_t s,
-                               bool pdl) {
+                               double temperature, const float *u, int32_t *picks, void *workspace, unsigned *flags,
+                               cudaStream_t s, bool pdl) {
   // CTAs per sequence: slices of at least 2048 entries, up to the largest cluster
   int CL = 1;
   while (CL < kSampleCluster && (long long)CL * 2048 < V) CL *= 2;
-  SampleArgs a{target, draft, drafts, u, picks, batch, k, V, 0, temperature, flags};
-  a.slice = ((V + CL - 1) / CL + 3) / 4 * 4;
-  cudaError_t e =
-      cudaFuncSetAttribute(spec_sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return e;
+  SampleArgs a{};
+  a.target = target;
+  a.draft = draft;
+  a.drafts = drafts;
+  a.u = u;
+  a.picks = picks;
+  a.batch = batch;
+  a.k = k;
+  a.V = V;
+  a.stats = reinterpret_cast<float2 *>(workspace);
+  a.chunks = sample_chunks(V);
+  a.slice = (V + CL - 1) / CL;
+  a.temperature = temperature;
+  a.flags = flags;
+  // both rows' weights where two CTAs then still share an SM, else one row's, else none
+  const size_t one = (size_t)a.slice * sizeof(double);
+  a.keep = k && 2 * one <= kKeepBytes / 2 ? 2 : one <= kKeepBytes ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(batch * CL));
-  cfg.blockDim = dim3(kSampleThreads);
   cfg.stream = s;
   cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)CL;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)CL;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
+  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.gridDim = dim3((unsigned)a.chunks, (unsigned)((2 * k + 1) * batch));
+  cfg.blockDim = dim3(kStatsThreads);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, sample_stats_kernel, a);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(spec_sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(spec_sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kKeepBytes);
+  if (e != cudaSuccess) return e;
+  cfg.attrs = pdl ? at : at + 1;
   cfg.numAttrs = pdl ? 2 : 1;
+  cfg.gridDim = dim3((unsigned)(batch * CL));
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = one * a.keep;
   return cudaLaunchKernelEx(&cfg, spec_sample_kernel, a);
 }
 

@@ -71,10 +71,15 @@ def spec_sample(target: torch.Tensor, draft: torch.Tensor | None, drafts: torch.
             raise _lib.GpuError(_lib.WG_INVALID_ARGUMENT, f"{what} must be contiguous {dt} on {device}")
     ctx = context(device.index)
     ctx.use_torch_stream()
+    L = _lib.lib()
+    need = ctypes.c_size_t()
+    ctx._check(L.wg_spec_sample_workspace(ctx.handle, batch, k, V, ctypes.byref(need)))
+    # from torch's allocator: safe on any stream and inside a graph
+    ws = torch.empty(max(need.value, 8), dtype=torch.uint8, device=device)
     with torch.cuda.device(device):
-        ctx._check(_lib.lib().wg_spec_sample(ctx.handle, target.data_ptr(), draft.data_ptr() if k else None,
-                                             drafts.data_ptr() if k else None, batch, k, V, temperature, u.data_ptr(),
-                                             out.data_ptr()))
+        ctx._check(L.wg_spec_sample(ctx.handle, target.data_ptr(), draft.data_ptr() if k else None,
+                                    drafts.data_ptr() if k else None, batch, k, V, temperature, u.data_ptr(),
+                                    out.data_ptr(), ws.data_ptr(), ws.numel()))
     return out
 
 
