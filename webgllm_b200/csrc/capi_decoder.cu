@@ -283,7 +283,7 @@ int wg_spec_sample(wg_ctx *ctx, const float *target, const float *draft, const i
                  workspace_bytes, need);
   return finish(ctx,
                 wg::launch_spec_sample(target, draft, drafts, batch, k, V, temperature, u, picks, workspace,
-                                       ctx->d_flags, ctx->stream, ctx->pdl),
+                                       ctx->d_flags, ctx->num_sms, ctx->stream, ctx->pdl),
                 "wg_spec_sample");
 }
 

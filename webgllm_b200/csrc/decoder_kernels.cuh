@@ -70,6 +70,6 @@ constexpr int kSampleMaxDrafts = 32, kSampleMaxVocab = 1 << 21;
 size_t spec_sample_workspace(int batch, int k, int V);
 cudaError_t launch_spec_sample(const float *target, const float *draft, const int32_t *drafts, int batch, int k, int V,
                                double temperature, const float *u, int32_t *picks, void *workspace, unsigned *flags,
-                               cudaStream_t s, bool pdl);
+                               int num_sms, cudaStream_t s, bool pdl);
 
 }  // namespace wg

@@ -11,10 +11,9 @@
 // (pieces of 8192 logits a CTA, all of its loads in flight at once) and leaves
 // (max, sum) of each piece in the workspace. spec_sample_kernel, a thread-block
 // cluster a sequence, (1) combines them, (2) decides acceptance, a lane a draft,
-// (3) makes the drawn row's weights in 64 bits, kept in shared memory where they
-// fit, a slice of the vocabulary a CTA, the CTAs' sums exchanged through
-// distributed shared memory, and (4) finds the token by the running sum over
-// CTAs, warps, lanes, and one lane's run. (In one launch, the clusters doing the
+// (3) makes the drawn row's weights in 64 bits, a slice of the vocabulary a CTA,
+// the CTAs' sums exchanged through distributed shared memory, and (4) finds the
+// token by the running sum over CTAs, warps, rounds of 256 and runs of 32. (In one launch, the clusters doing the
 // streaming too, 61 sequences of 11 rows of 65543 took 144 us: their phases run
 // in step, and the memory idles through the later ones.)
 // The answer is a whole number, so it must not hang on rounding. The
@@ -24,7 +23,7 @@
 // throughout: p - q cancels where draft and target agree, and its running sum
 // is compared with u at a resolution of one token in V.
 // Bound: the (2k + 1) V logits of a sequence, read once (HBM), plus the 64-bit
-// exponentials of the drawn rows (3 V a sequence, 12 operations each).
+// exponentials of the drawn rows (V to 4 V a sequence, 10 operations each).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -37,9 +36,8 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kSampleThreads = 512;
-constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleCluster = 16;  // largest cluster
+constexpr int kSlots = 64;
 constexpr size_t kKeepBytes = 200 * 1024;  // of shared memory for the drawn rows' weights
 constexpr int kMaxRows = 2 * kSampleMaxDrafts + 1;
 // Relative error bound of u q(d) / p(d) when the two normalising sums come from
@@ -59,8 +57,9 @@ struct SampleArgs {
   float2 *stats;          // [2k + 1][batch][chunks]: (max, sum) of a row's pieces
   int chunks;
   int slice;              // vocabulary entries per CTA
-  int keep;               // arrays of the slice's weights kept in shared memory: p's, then q's
-  double temperature;
+  int keep;               // whether both rows' weights of the slice are kept in shared memory
+  float log2_scale;       // log2 e / T
+  double scale, span;     // 16 log2 e / T; 990 octaves as a difference of logits
   unsigned *flags;
 };
 
@@ -84,13 +83,14 @@ __device__ __forceinline__ double last16(double scanned) { return __shfl_sync(0x
 
 // The sum of one double per thread over the CTA, the same bits in every thread;
 // `warp_part` afterwards holds the warps' sums.
+template <int kWarps>
 __device__ __forceinline__ double cta_sum(double v, double *warp_part) {
   v = warp_sum_f64(v);
   __syncthreads();
   const int lane = threadIdx.x & 31;
   if (lane == 0) warp_part[threadIdx.x >> 5] = v;
   __syncthreads();
-  return last16(scan16(warp_part[lane & 15], lane));
+  return last16(scan16((lane & 15) < kWarps ? warp_part[lane & 15] : 0.0, lane));
 }
 
 // The running sums of the cluster's CTAs (their *mine), the same bits in every
@@ -100,11 +100,12 @@ __device__ __forceinline__ double ranks_scan(const double *mine, int lane, int C
   const int i = lane & 15;
   return scan16(i < CL ? *cg::this_cluster().map_shared_rank(mine, i) : 0.0, lane);
 }
-// exp((x - max) / T) in 64 bits, off by less than 2^-50: 2^(n / 16) from a
+// exp((x - max) / T) in 64 bits, off by less than 2^-47: 2^(n / 16) from a
 // table (16 doubles in shared memory: one bank row, no conflicts whatever the
-// lanes pick), n the nearest to 16 log2 e (x - max) / T, times the Taylor
-// polynomial of the rest (at most ln 2 / 32 away: degree 7 leaves 2e-18).
-// Below 2^-1000: 0.
+// lanes pick), n the nearest to 16 log2 e (x - max) / T, times the polynomial of
+// degree 5 through 2^(f / 16) at the six Chebyshev points of |f| <= 1/2 (off by
+// 4.6e-15). Ten 64-bit operations and no branch: the 64-bit pipe (a warp's
+// operation every 2.8 cycles) bounds these passes. Below 2^-990 and at -inf: 0.
 __constant__ double kRoots[16] = {
     1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
     1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
@@ -112,25 +113,23 @@ __constant__ double kRoots[16] = {
     1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
 struct Exp64 {
   double scale, shift;  // 16 log2 e / T, and - max times it
+  float low, max;       // logits at or below `low` have weight 0
   const double *table;
   __device__ __forceinline__ double operator()(float x) const {
-    const double y = fma((double)x, scale, shift);
-    if (!(y > -16000.0)) return 0.0;
-    const double t = y + 6755399441055744.0;  // n in the low bits
+    // (a hidden logit as the maximum, times the table's 17th entry, 0)
+    const bool some = x > low;
+    const double xd = (double)(some ? x : max);
+    const double t = fma(xd, scale, shift + 6755399441055744.0);  // n in the low bits
     const int n = __double2loint(t);
-    const double f = y - (t - 6755399441055744.0);
-    constexpr double h = 0.04332169878499658;  // ln 2 / 16
-    constexpr double h2 = h * h, h3 = h2 * h, h4 = h2 * h2;
-    double p = h4 * h3 / 5040.0;
-    p = fma(p, f, h3 * h3 / 720.0);
-    p = fma(p, f, h3 * h2 / 120.0);
-    p = fma(p, f, h4 / 24.0);
-    p = fma(p, f, h3 / 6.0);
-    p = fma(p, f, h2 / 2.0);
-    p = fma(p, f, h);
-    p = fma(p, f, 1.0);
-    const double r = p * table[n & 15];
-    return __hiloint2double(__double2hiint(r) + ((n >> 4) << 20), __double2loint(r));
+    const double f = fma(xd, scale, shift - (t - 6755399441055744.0));
+    double p = 0x1.5d897e525c216p-30;
+    p = fma(p, f, 0x1.3b2c9b8a6caeap-23);
+    p = fma(p, f, 0x1.c6b08d6f2a289p-17);
+    p = fma(p, f, 0x1.ebfbdff555824p-11);
+    p = fma(p, f, 0x1.62e42fefa39f3p-5);
+    p = fma(p, f, 0x1.0000000000014p+0);
+    const double r = p * table[some ? n & 15 : 16];
+    return __hiloint2double(__double2hiint(r) + (n & ~15) * 65536, __double2loint(r));
   }
 };
 
@@ -145,7 +144,7 @@ __global__ void __launch_bounds__(kStatsThreads) sample_stats_kernel(const Sampl
   const int tid = threadIdx.x, lane = tid & 31, V = a.V;
   const int rows_t = (a.k + 1) * a.batch, r = blockIdx.y;
   const float *p = r < rows_t ? a.target + (size_t)r * V : a.draft + (size_t)(r - rows_t) * V;
-  const float c = (float)(1.4426950408889634 / a.temperature);
+  const float c = a.log2_scale;
   // the piece's aligned float4s; the row's ends (fewer than 4 logits each) go to
   // its first and its last piece
   const int lead = min((int)((4 - ((uintptr_t)p >> 2 & 3)) & 3), V), quads = (V - lead) / 4;
@@ -187,35 +186,37 @@ __global__ void __launch_bounds__(kStatsThreads) sample_stats_kernel(const Sampl
   }
 }
 
-__global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const SampleArgs a) {
+template <int kWarps, int kCtasPerSm>
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) spec_sample_kernel(const SampleArgs a) {
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), CL = (int)cl.num_blocks();
   const int b = blockIdx.x / CL;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int k = a.k, R = 2 * k + 1, V = a.V;
-  extern __shared__ __align__(16) double kept[];  // [keep][slice] weights of the drawn row
+  extern __shared__ __align__(16) double kept[];  // weights of the drawn row: p's, then q's (a.keep)
   __shared__ float row_m[kMaxRows];
   __shared__ double row_z[kMaxRows];
-  __shared__ double table[16], warp_part[kSampleWarps], cta_part[4];
+  __shared__ double table[17], warp_part[kWarps], cta_part[4];
+  __shared__ double slots[kWarps][kSlots];  // each warp's sums of the draw's weights, by rounds
   __shared__ int s_n, s_owner;
-  static_assert(kSampleWarps == 16 && kSampleCluster == 16, "16 lanes scan");
+  static_assert(kWarps <= 16 && kSampleCluster == 16, "16 lanes scan");
 
   pdl_trigger();
-  if (tid < 16) table[tid] = kRoots[tid];
+  if (tid < 17) table[tid] = tid < 16 ? kRoots[tid] : 0.0;
   pdl_wait();
 
   // rows 0 .. k: the target's; k + 1 .. 2k: the draft's
   auto row = [&](int r) {
     return r <= k ? a.target + ((size_t)r * a.batch + b) * V : a.draft + ((size_t)(r - k - 1) * a.batch + b) * V;
   };
-  const float c = (float)(1.4426950408889634 / a.temperature);
+  const float c = a.log2_scale;
 
   // ---- (1) every row's maximum and sum, from its pieces'; meanwhile the last
   // warp fetches what acceptance needs (lane j: draft j)
   int d = -1;
   float xp_d = 0.0f, xq_d = 0.0f;
   double u_d = 0.0;
-  if (warp == kSampleWarps - 1 && lane < k) {
+  if (warp == kWarps - 1 && lane < k) {
     d = a.drafts[(size_t)b * k + lane];
     u_d = (double)a.u[(size_t)b * (k + 1) + lane];
     if (u_d >= 1.0) u_d = 1.0 - 0x1p-24;
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const Sa
       xq_d = row(k + 1 + lane)[d];
     }
   }
-  for (int r = warp; r < R; r += kSampleWarps) {
+  for (int r = warp; r < R; r += kWarps) {
     const float2 *st = a.stats + ((size_t)r * a.batch + b) * a.chunks;
     float2 v = lane < a.chunks ? __ldcg(st + lane) : make_float2(-INFINITY, 0.0f);
     float m = v.x;
@@ -244,22 +245,24 @@ __global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const Sa
   __syncthreads();
 
   const int v0 = (int)min((long long)V, (long long)rank * a.slice), n_v = (int)min((long long)a.slice, (long long)V - v0);
-  // this warp's run of the slice; each lane a run of it, of odd length (the
-  // lanes then meet no bank conflicts)
-  const int per_lane = (n_v + kSampleThreads - 1) / kSampleThreads | 1;
-  const int w0 = min(n_v, warp * 32 * per_lane), w1 = min(n_v, w0 + 32 * per_lane);
-  const int l0 = min(w1, w0 + lane * per_lane), l1 = min(w1, l0 + per_lane);
-  const double scale = 16.0 * 1.4426950408889634074 / a.temperature;
-  auto weights = [&](int r) { return Exp64{scale, -(double)row_m[r] * scale, table}; };
-  // f(i, logit) over this warp's run of a row, eight loads a lane in flight
+  // this warp's run of the slice, in rounds of 256 (8 logits a lane, 32 apart)
+  const int per_warp = (n_v + 256 * kWarps - 1) / (256 * kWarps) * 256;
+  const int w0 = min(n_v, warp * per_warp), w1 = min(n_v, w0 + per_warp);
+  auto weights = [&](int r) {
+    const double m = (double)row_m[r], low = m - a.span;
+    return Exp64{a.scale, -m * a.scale, low > -3.4e38 ? (float)low : -3.4e38f, row_m[r], table};
+  };
+  auto round_of = [&](const float *x, int i0, float v[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = i0 + 32 * e < w1 ? __ldg(x + i0 + 32 * e) : -INFINITY;
+  };
+  // f(i, logit) over this warp's run of a row (-inf past its end)
   auto each = [&](const float *x, auto &&f) {
-    for (int i0 = w0 + lane; i0 < w1; i0 += 256) {
+    for (int i0 = w0 + lane; i0 < w1 + lane; i0 += 256) {
       float v[8];
+      round_of(x, i0, v);
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = i0 + 32 * e < w1 ? __ldg(x + i0 + 32 * e) : 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (i0 + 32 * e < w1) f(i0 + 32 * e, v[e]);
+      for (int e = 0; e < 8; e++) f(i0 + 32 * e, v[e]);
     }
   };
   // the sum of row r's weights over the whole vocabulary
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const Sa
     const Exp64 w = weights(r);
     double s = 0.0;
     each(row(r) + v0, [&](int, float x) { s += w(x); });
-    s = cta_sum(s, warp_part);
+    s = cta_sum<kWarps>(s, warp_part);
     if (tid == 0) cta_part[0] = s;
     cl.sync();
     s = last16(ranks_scan(&cta_part[0], lane, CL));
@@ -278,7 +281,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const Sa
   // ---- (2) acceptance: lane j decides draft j, the same in every CTA
   int n = 0;
   if (k > 0) {
-    if (warp == kSampleWarps - 1) {
+    if (warp == kWarps - 1) {
       bool kept_it = false, close = false;
       if (lane < k && d >= 0 && d < V) {
         const double lhs = u_d * weights(k + 1 + lane)(xq_d) * row_z[lane];
@@ -313,7 +316,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const Sa
 
   // rows without probabilities (NaN, +inf, -inf throughout): a token all the
   // same, never the rejected one, and a report
-  const int dn = n < k ? a.drafts[(size_t)b * k + n] : -1;
+  const int dn = n < k ? a.drafts[(size_t)b * k + n] : -1;  // (-1: no token is left out)
   auto is_row = [&](int r) { return row_z[r] > 0.0 && row_z[r] < INFINITY; };
   auto report = [&]() {
     if (rank == 0 && tid == 0) {
@@ -336,21 +339,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const Sa
   const float *xp = row(n) + v0, *xq = diff ? row(k + 1 + n) + v0 : nullptr;
   const Exp64 wp = weights(n), wq = weights(diff ? k + 1 + n : n);
   double ip = 1.0, iq = 0.0;
-  double *const kept_q = kept + a.slice;
+  double *const kept_q = kept + (a.slice + 255) / 256 * 256;
   if (diff) {
     double sp = 0.0, sq = 0.0;
-    each(xq, [&](int i, float x) {
-      const double e = wq(x);
-      if (a.keep == 2) kept_q[i] = e;
-      sq += e;
-    });
-    each(xp, [&](int i, float x) {
-      const double e = wp(x);
-      if (a.keep) kept[i] = e;
-      sp += e;
-    });
-    sp = cta_sum(sp, warp_part);
-    sq = cta_sum(sq, warp_part);
+    for (int i0 = w0 + lane; i0 < w1 + lane; i0 += 256) {
+      float x[8], y[8];
+      round_of(xp, i0, x);
+      round_of(xq, i0, y);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const double ep = wp(x[e]), eq = wq(y[e]);
+        if (a.keep) {
+          kept[i0 + 32 * e] = ep;
+          kept_q[i0 + 32 * e] = eq;
+        }
+        sp += ep;
+        sq += eq;
+      }
+    }
+    sp = cta_sum<kWarps>(sp, warp_part);
+    sq = cta_sum<kWarps>(sq, warp_part);
     if (tid == 0) {
       cta_part[1] = sp;
       cta_part[2] = sq;
@@ -359,39 +367,50 @@ __global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const Sa
     const double rp = ranks_scan(&cta_part[1], lane, CL), rq = ranks_scan(&cta_part[2], lane, CL);
     ip = 1.0 / last16(rp);
     iq = 1.0 / last16(rq);
-    // (where only p's weights fit, q's are made a second time)
-    if (a.keep == 1) each(xq, [&](int i, float x) { kept[i] = fmax(kept[i] * ip - wq(x) * iq, 0.0); });
-  } else if (a.keep) {
-    each(xp, [&](int i, float x) { kept[i] = wp(x); });
   }
-  __syncwarp();
   bool without = false;  // p without the rejected token instead
-  auto mass = [&](int i) {
-    if (without) return v0 + i == dn ? 0.0 : wp(xp[i]);
-    if (a.keep == 2) return diff ? fmax(kept[i] * ip - kept_q[i] * iq, 0.0) : kept[i];
-    if (a.keep == 1) return kept[i];
-    return diff ? fmax(wp(xp[i]) * ip - wq(xq[i]) * iq, 0.0) : wp(xp[i]);
+  // what each of a lane's 8 tokens i0, i0 + 32, ... of a round weighs
+  auto masses = [&](int i0, double m[8]) {
+    float v[8];
+    if (diff && a.keep && !without) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) m[e] = fmax(kept[i0 + 32 * e] * ip - kept_q[i0 + 32 * e] * iq, 0.0);
+      return;
+    }
+    round_of(xp, i0, v);
+    if (diff && !without) {
+      float y[8];
+      round_of(xq, i0, y);
+#pragma unroll
+      for (int e = 0; e < 8; e++) m[e] = fmax(wp(v[e]) * ip - wq(y[e]) * iq, 0.0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) m[e] = v0 + i0 + 32 * e == dn ? 0.0 : wp(v[e]);
+    }
   };
 
   // ---- (4) the token: the first whose running sum exceeds u times the total
-  double total, before, after, lane_sum, lane_head;
+  double total, before, after, warp_total, warp_head;
+  const int per_slot = (per_warp / 256 + kSlots - 1) / kSlots * 256;  // rounds that share a slot
   for (;;) {
-    lane_sum = 0.0;
-    for (int i = l0; i < l1; i++) lane_sum += mass(i);
-    double s = lane_sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double t = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += t;
+    warp_total = 0.0;
+    for (int slot = 0, i0 = w0; i0 < w1; slot++) {
+      double s = 0.0;
+      for (const int i1 = min(w1, i0 + per_slot); i0 < i1; i0 += 256) {
+        double m[8];
+        masses(i0 + lane, m);
+        s += ((m[0] + m[1]) + (m[2] + m[3])) + ((m[4] + m[5]) + (m[6] + m[7]));
+      }
+      s = warp_sum_f64(s);
+      if (lane == 0) slots[warp][slot] = s;
+      warp_total += s;
     }
-    lane_head = __shfl_up_sync(0xffffffffu, s, 1);
-    if (lane == 0) lane_head = 0.0;
     __syncthreads();
-    if (lane == 31) warp_part[warp] = s;
+    if (lane == 0) warp_part[warp] = warp_total;
     if (tid == 0) s_owner = -1;
     __syncthreads();
-    const double warps = scan16(warp_part[lane & 15], lane);
-    if (warp > 0) lane_head += __shfl_sync(0xffffffffu, warps, warp - 1);
+    const double warps = scan16((lane & 15) < kWarps ? warp_part[lane & 15] : 0.0, lane);
+    warp_head = warp > 0 ? __shfl_sync(0xffffffffu, warps, warp - 1) : 0.0;
     if (tid == 15) cta_part[3] = warps;
     cl.sync();
     const double ranks = ranks_scan(&cta_part[3], lane, CL);
@@ -410,24 +429,64 @@ __global__ void __launch_bounds__(kSampleThreads, 2) spec_sample_kernel(const Sa
   if (!(u > 0.0)) u = 0.0;
   const double goal = u * total;
   if (!(total > 0.0)) report();  // all of p on the rejected token: q was no distribution
-  // One CTA holds the goal. There the running sum at the head of every lane's
-  // run says which lane: the last one that has weight and whose head is not past
-  // the goal.
+  // One CTA holds the goal. There: the last warp that has weight and whose head
+  // is not past the goal, in it the last round, there the last run of 32, and in
+  // that the first token past the goal. (Where rounding leaves the goal past the
+  // run's own sum: its last token with weight.)
   if (total > 0.0 && before <= goal && goal < after) {
-    double head = before + lane_head;
-    const unsigned here = __ballot_sync(0xffffffffu, lane_sum > 0.0 && head <= goal);
-    if (here && lane == 0) atomicMax(&s_owner, warp * 32 + 31 - __clz(here));
+    double head = before + warp_head;
+    if (lane == 0 && warp_total > 0.0 && head <= goal) atomicMax(&s_owner, warp);
     __syncthreads();
-    if (tid == s_owner) {
-      int pick = -1;
-      for (int i = l0; i < l1; i++) {
-        const double m = mass(i);
-        if (!(m > 0.0)) continue;
-        pick = i;  // (rounding may leave the goal past the run's own sum: its last weight then)
-        head += m;
-        if (head > goal) break;
+    if (warp == s_owner) {
+      int at = w0;
+      double at_head = head, m[8];
+      for (int slot = 0, i0 = w0; i0 < w1; slot++, i0 += per_slot) {
+        const double s = slots[warp][slot];
+        if (s > 0.0 && head <= goal) {
+          at = i0;
+          at_head = head;
+        }
+        head += s;
       }
-      a.picks[(size_t)n * a.batch + b] = v0 + pick;
+      if (per_slot > 256) {  // (a vocabulary a warp: the slot's rounds once more)
+        head = at_head;
+        for (int i0 = at, i1 = min(w1, at + per_slot); i0 < i1; i0 += 256) {
+          masses(i0 + lane, m);
+          const double s =
+              warp_sum_f64(((m[0] + m[1]) + (m[2] + m[3])) + ((m[4] + m[5]) + (m[6] + m[7])));
+          if (s > 0.0 && head <= goal) {
+            at = i0;
+            at_head = head;
+          }
+          head += s;
+        }
+      }
+      masses(at + lane, m);
+      double sums[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) sums[e] = warp_sum_f64(m[e]);
+      head = at_head;
+      double run = 0.0, run_head = head;
+      int run_at = at;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (sums[e] > 0.0 && head <= goal) {
+          run = m[e];
+          run_head = head;
+          run_at = at + 32 * e;
+        }
+        head += sums[e];
+      }
+      double s = run;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, run > 0.0 && run_head + s > goal);
+      const unsigned some = __ballot_sync(0xffffffffu, run > 0.0);
+      if (lane == 0)
+        a.picks[(size_t)n * a.batch + b] = v0 + run_at + (past ? __ffs(past) - 1 : 31 - __clz(some));
     }
   }
   cl.sync();  // peers may still read this CTA's shared memory
@@ -443,10 +502,15 @@ size_t spec_sample_workspace(int batch, int k, int V) {
 
 cudaError_t launch_spec_sample(const float *target, const float *draft, const int32_t *drafts, int batch, int k, int V,
                                double temperature, const float *u, int32_t *picks, void *workspace, unsigned *flags,
-                               cudaStream_t s, bool pdl) {
-  // CTAs per sequence: slices of at least 2048 entries, up to the largest cluster
+                               int num_sms, cudaStream_t s, bool pdl) {
+  // CTAs per sequence: as many as leave slices of 4096 entries, and no more than
+  // let all sequences run at once (61 sequences of 65543, k = 5: 8 CTAs each 66
+  // us, 4 or 16 CTAs 82 and 79 us)
   int CL = 1;
-  while (CL < kSampleCluster && (long long)CL * 2048 < V) CL *= 2;
+  while (CL < kSampleCluster && (long long)CL * 4096 < V && (long long)batch * CL * 2 <= 4 * num_sms) CL *= 2;
+  // 16 warps a CTA where it has an SM to itself and work for them (8 sequences of
+  // 128256, k = 4: 22 us, with 8 warps 28 us), else 8
+  const bool wide = batch * CL <= num_sms && (V + CL - 1) / CL >= 4096;
   SampleArgs a{};
   a.target = target;
   a.draft = draft;
@@ -459,11 +523,14 @@ cudaError_t launch_spec_sample(const float *target, const float *draft, const in
   a.stats = reinterpret_cast<float2 *>(workspace);
   a.chunks = sample_chunks(V);
   a.slice = (V + CL - 1) / CL;
-  a.temperature = temperature;
+  a.log2_scale = (float)(1.4426950408889634 / temperature);
+  a.scale = 16.0 * 1.4426950408889634074 / temperature;
+  a.span = 15840.0 / a.scale;
   a.flags = flags;
-  // both rows' weights where two CTAs then still share an SM, else one row's, else none
-  const size_t one = (size_t)a.slice * sizeof(double);
-  a.keep = k && 2 * one <= kKeepBytes / 2 ? 2 : one <= kKeepBytes ? 1 : 0;
+  // A rejected sequence's weights are used twice: kept where that costs no other
+  // CTA its place (each SM has one at most), made again otherwise
+  const size_t weights = 2 * (size_t)((a.slice + 255) / 256 * 256) * sizeof(double);
+  a.keep = k && weights <= kKeepBytes && wide;
   cudaLaunchConfig_t cfg = {};
   cfg.stream = s;
   cudaLaunchAttribute at[2];
@@ -478,17 +545,17 @@ cudaError_t launch_spec_sample(const float *target, const float *draft, const in
   cfg.gridDim = dim3((unsigned)a.chunks, (unsigned)((2 * k + 1) * batch));
   cfg.blockDim = dim3(kStatsThreads);
   cudaError_t e = cudaLaunchKernelEx(&cfg, sample_stats_kernel, a);
+  auto kern = wide ? spec_sample_kernel<16, 1> : spec_sample_kernel<8, 4>;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(spec_sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(spec_sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kKeepBytes);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kKeepBytes);
   if (e != cudaSuccess) return e;
   cfg.attrs = pdl ? at : at + 1;
   cfg.numAttrs = pdl ? 2 : 1;
   cfg.gridDim = dim3((unsigned)(batch * CL));
-  cfg.blockDim = dim3(kSampleThreads);
-  cfg.dynamicSmemBytes = one * a.keep;
-  return cudaLaunchKernelEx(&cfg, spec_sample_kernel, a);
+  cfg.blockDim = dim3(wide ? 512 : 256);
+  cfg.dynamicSmemBytes = a.keep ? weights : 0;
+  return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 }  // namespace wg
