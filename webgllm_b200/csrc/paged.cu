@@ -179,28 +179,33 @@ __global__ void __launch_bounds__(256)
 // o = softmax(q k^T) v per (sequence, KV head, 16 MT rows of queries), where
 // the sequence's rows times the G query heads of the KV head are the rows of
 // one small matrix product: a K / V tile is read once for all of them. Decode
-// is bound by those reads, so the work is counted in tiles of 64 keys over
+// is bound by those reads, so the work is counted in tiles of 4 KW keys over
 // all sequences and heads and each of P resident CTAs takes an equal run of
 // tiles, wherever sequences begin and end in it: short and long sequences
 // share the machine evenly whatever their lengths, which only the device
 // knows. Per CTA:
-//   warp 4      the producer: page entries, then one TMA copy per box of a
-//               page's rows x 64 dims (128-byte swizzle) into a ring of
-//               stages (K and V of 64 keys each);
-//   warps 0-3   16 keys of a tile each, for all its query rows: S = Q K^T and
-//               O += P V on mma.m16n8k16 with fp32 sums, a running maximum
-//               and sum per row in registers (log2 domain). The warps meet
-//               only at the end of a run of tiles.
+//   the last warp   the producer: page entries, then one TMA copy per box of a
+//                   page's rows x 64 dims (128-byte swizzle) into a ring of
+//                   stages (K and V of a tile each);
+//   4 MT warps      KW keys of a tile and 16 of the query rows each: S = Q K^T
+//                   and O += P V on mma.m16n8k16 with fp32 sums, a running
+//                   maximum and sum per row in registers (log2 domain). The
+//                   warps meet only at the end of a run of tiles. A tile's chain
+//                   (wait, scores, maximum, exponentials, P V) takes a warp
+//                   about 2000 cycles whatever KW is, so small heads take 32
+//                   keys at a time (Dh = 64, 32 sequences with a window of 4096:
+//                   WIN16 us with 16 keys, WIN32 us with 32), and 32 query rows
+//                   take eight warps (five rows of 4 heads, 8 sequences of 4k:
+//                   VER4 us with four warps of both row tiles, VER8 us).
 // P stays at fp32 precision: hi + lo 16-bit halves, two products (the tensor
 // pipe idles under the loads).
 // A (sequence, head, rows) unit that one CTA finishes alone is written by it;
 // else each CTA leaves (max, sum, O) in the workspace and paged_join_kernel
 // adds them in order: no atomics, the same bits every time.
 
-constexpr int kKeys = 64;          // keys per tile
-constexpr int kSplitWarps = 4;     // consumer warps (16 keys each)
-constexpr int kSplitThreads = (kSplitWarps + 1) * 32;
 constexpr int kMaxStages = 8;
+// A CTA takes at least this many keys, or one tile.
+constexpr int kMinKeys = 64;
 
 struct SplitArgs {
   PagedRows pr;
@@ -209,7 +214,7 @@ struct SplitArgs {
   void *out;
   int H, Hkv, G;
   int window, sinks;
-  int box_rows;  // keys of one TMA box: divides page_size and 64
+  int box_rows;  // keys of one TMA box: divides page_size and the tile
   int stages;
   int *rec;      // workspace: [P][8]
   float *part;   // workspace: [2 P][rows * (Dh + 2)]
@@ -223,12 +228,12 @@ struct SeqWork : KeySpan {
   int mt;     // row tiles
 };
 
-__device__ __forceinline__ SeqWork seq_work(const SplitArgs &A, int b, int rows_per_tile) {
+__device__ __forceinline__ SeqWork seq_work(const SplitArgs &A, int b, int rows_per_tile, int tile_keys) {
   SeqWork w;
   seq_rows(A.pr, b, w.r0, w.n);
   w.p = A.pr.pos[b];
   w.mt = (int)(((long long)w.n * A.G + rows_per_tile - 1) / rows_per_tile);
-  static_cast<KeySpan &>(w) = key_span(w.p, w.n, A.window, A.sinks, A.pt, kKeys);
+  static_cast<KeySpan &>(w) = key_span(w.p, w.n, A.window, A.sinks, A.pt, tile_keys);
   return w;
 }
 
@@ -251,46 +256,63 @@ __device__ __forceinline__ int block_scan_incl(int v, int *red, int &total) {
   return v + before;
 }
 
-template <typename T, int Dh, int MT>
-struct SplitSmem {
+template <int Dh_, int MT>
+struct SplitCfg {
+  static constexpr int Dh = Dh_;
+  static constexpr int KW = Dh == 64 ? 32 : 16;    // keys of a warp
+  static constexpr int kKeys = 4 * KW;             // of a tile
   static constexpr int kRows = 16 * MT;
+  static constexpr int kWarps = 4 * MT;            // consumers
+  static constexpr int kThreads = (kWarps + 1) * 32;
+  static constexpr int kCtas = MT == 1 && Dh <= 128 ? 2 : 1;  // per SM
   static constexpr int kTileBytes = kKeys * Dh * 2;  // K or V of a stage
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kRedBytes = 2 * kRows * Dh * 4;  // the warps' merge
-  static constexpr int kFixed = 1024 /* alignment */ + kRedBytes + 4 * kSplitWarps * kRows * 2 + 256;
+  // The warps' merge: two sets of the rows' sums, 8 floats between rows (the 8
+  // rows a warp writes at once then meet in 2 bank rounds instead of 8). The
+  // same memory stages the queries, and P where a V row is odd.
+  static constexpr int kRedRow = Dh + 8;
+  static constexpr int kRedBytes = 2 * kRows * kRedRow * 4;
+  static constexpr int kFixed = 1024 /* alignment */ + kRedBytes + 4 * 4 * kRows * 2 + 256;
+  static constexpr int kBudget = 224 * 1024 / kCtas - 1024;
+  static constexpr int kFit = (kBudget - kFixed) / kStageBytes;
+  static constexpr int kStages = kFit > kMaxStages ? kMaxStages : kFit;
+  static constexpr int kSmem = kStages * kStageBytes + kFixed;
+  static_assert(kStages >= 2, "two stages");
+  static_assert(kRedBytes >= kWarps * 16 * KW * 4 && kRedBytes >= kRows * (Dh + 8) * 2, "the merge buffer's other uses");
 };
 
 template <typename T, int Dh, int MT>
-__global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::kCtas)
     paged_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const SplitArgs A) {
-  using S = SplitSmem<T, Dh, MT>;
+  using C = SplitCfg<Dh, MT>;
+  constexpr int KW = C::KW, kKeys = C::kKeys, S = C::kStages;
   constexpr int kBlk = Dh / 64;                    // 64-dim blocks of a row
   constexpr int kBlkBytes = kKeys * 128;           // one block of a stage's K or V
   constexpr float kLog2e = 1.4426950408889634f;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  float *red = reinterpret_cast<float *>(smem + (size_t)A.stages * S::kStageBytes);  // [2][kRows][Dh]
-  float *sm_m = red + 2 * S::kRows * Dh;           // [warps][kRows]
-  float *sm_l = sm_m + kSplitWarps * S::kRows;
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages];
-  __shared__ int held[kMaxStages];                 // which of a stage's boxes were loaded
-  __shared__ int scan_red[kSplitThreads / 32];
+  float *red = reinterpret_cast<float *>(smem + (size_t)S * C::kStageBytes);  // [2][kRows][kRedRow]
+  float *sm_m = red + 2 * C::kRows * C::kRedRow;           // [4 key groups][kRows]
+  float *sm_l = sm_m + 4 * C::kRows;
+  __shared__ uint64_t full[S], empty[S];
+  __shared__ int held[S];                          // which 16-key groups of a stage's pages were loaded
+  __shared__ int scan_red[C::kThreads / 32];
   __shared__ int s_b, s_base, aborted;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int P = (int)gridDim.x, cta = (int)blockIdx.x;
 
   if (tid == 0) {
-    for (int i = 0; i < A.stages; i++) {
+    for (int i = 0; i < S; i++) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kSplitWarps);
+      mbar_init(&empty[i], C::kWarps);
     }
     fence_mbar_init();
     aborted = 0;
     s_b = A.pr.batch;
     s_base = 0;
   }
-  if (warp == kSplitWarps && lane == 0) {
+  if (warp == C::kWarps && lane == 0) {
     prefetch_tensormap(&tm_k);
     prefetch_tensormap(&tm_v);
   }
@@ -298,55 +320,79 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
   pdl_wait();  // rows, positions, pages and queries come from earlier kernels
   __syncthreads();
 
-  // the total work, then where this CTA's run begins
-  int total = 0;
-  for (int b0 = 0; b0 < A.pr.batch; b0 += kSplitThreads) {
-    int v = 0, t;
-    if (b0 + tid < A.pr.batch) {
-      const SeqWork w = seq_work(A, b0 + tid, S::kRows);
-      v = A.Hkv * w.mt * w.nt;
+  // the total work, then where this CTA's run begins: by every warp itself for
+  // up to 32 sequences, else by the CTA, in passes of a thread a sequence
+  int total = 0, b = A.pr.batch, base = 0, per, start, end;
+  auto share = [&]() {
+    per = max((total + P - 1) / P, max(1, kMinKeys / kKeys));
+    start = (int)min((long long)total, (long long)cta * per);
+    end = (int)min((long long)total, (long long)start + per);
+  };
+  auto work_of = [&](int i) {
+    if (i >= A.pr.batch) return 0;
+    const SeqWork w = seq_work(A, i, C::kRows, kKeys);
+    return A.Hkv * w.mt * w.nt;
+  };
+  if (A.pr.batch <= 32) {
+    const int v = work_of(lane);
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
     }
-    block_scan_incl(v, scan_red, t);
-    total += t;
+    total = __shfl_sync(0xffffffffu, incl, 31);
+    share();
+    const unsigned at = __ballot_sync(0xffffffffu, incl - v <= start && start < incl);
+    if (at) {
+      b = __ffs(at) - 1;
+      base = __shfl_sync(0xffffffffu, incl - v, b);
+    }
+  } else {
+    int v = 0, incl = 0, t;
+    for (int b0 = 0; b0 < A.pr.batch; b0 += C::kThreads) {
+      v = work_of(b0 + tid);
+      incl = block_scan_incl(v, scan_red, t);
+      total += t;
+    }
+    share();
+    for (int b0 = 0, run = 0; b0 < A.pr.batch && run <= start; b0 += C::kThreads) {
+      if (A.pr.batch > C::kThreads) {
+        v = work_of(b0 + tid);
+        incl = run + block_scan_incl(v, scan_red, t);
+      }
+      if (incl - v <= start && start < incl) {
+        s_b = b0 + tid;
+        s_base = incl - v;
+      }
+      run += t;
+    }
+    __syncthreads();
+    b = s_b;
+    base = s_base;
   }
-  const int per = (total + P - 1) / P;
-  const int start = min((long long)total, (long long)cta * per), end = min((long long)total, (long long)start + per);
-  for (int b0 = 0, run = 0; b0 < A.pr.batch && run <= start; b0 += kSplitThreads) {
-    int v = 0, t;
-    if (b0 + tid < A.pr.batch) {
-      const SeqWork w = seq_work(A, b0 + tid, S::kRows);
-      v = A.Hkv * w.mt * w.nt;
-    }
-    const int incl = run + block_scan_incl(v, scan_red, t);
-    if (incl - v <= start && start < incl) {
-      s_b = b0 + tid;
-      s_base = incl - v;
-    }
-    run += t;
-  }
-  __syncthreads();
-  int b = s_b, base = s_base;
 
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    if (*(volatile int *)&aborted) return;
+    if (mbar_try_wait(bar, parity) || *(volatile int *)&aborted) return;
     if (!mbar_wait_bounded(bar, parity, A.flags)) *(volatile int *)&aborted = 1;
   };
   int stage = 0, phase = 0;
   auto advance = [&]() {
-    if (++stage == A.stages) {
+    if (++stage == S) {
       stage = 0;
       phase ^= 1;
     }
   };
 
-  if (warp == kSplitWarps) {
+  if (warp == C::kWarps) {
     // ---- producer ----
     const int nb = kKeys / A.box_rows;  // boxes per tile
     const int nops = nb * kBlk * 2;
     const int box = lane % nb, blk = (lane / nb) % kBlk, is_v = lane / (nb * kBlk);
     const uint32_t box_bytes = (uint32_t)A.box_rows * 128;
+    const int groups = A.box_rows / 16, gmask = (1 << groups) - 1;
     for (int pos = start; pos < end;) {
-      const SeqWork w = seq_work(A, b, S::kRows);
+      const SeqWork w = seq_work(A, b, C::kRows, kKeys);
       const int work = A.Hkv * w.mt * w.nt;
       if (pos >= base + work) {
         base += work;
@@ -363,8 +409,8 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
         seen = lane < nops && key < w.hi && (key < w.se || key + A.box_rows > w.ws);
         return seen ? row[key / A.pt.page_size] : -1;
       };
-      int key, key_next;
-      bool seen, seen_next;
+      int key, key_next = 0;
+      bool seen, seen_next = false;
       int page = entry(t0, key, seen), page_next = -1;
       for (int t = t0; t < t1; t++) {
         if (t + 1 < t1) page_next = entry(t + 1, key_next, seen_next);
@@ -373,16 +419,16 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
         if (seen && !ok) raise_flag(A.flags, kFlagBadArgument);
         const unsigned loaded = __ballot_sync(0xffffffffu, ok && lane < nb);
         if (lane == 0) {
-          held[stage] = (int)loaded;
+          int m = 0;
+          for (int i = 0; i < nb; i++)
+            if (loaded >> i & 1) m |= gmask << (i * groups);
+          held[stage] = m;
           mbar_expect_tx(&full[stage], (uint32_t)__popc(loaded) * box_bytes * kBlk * 2);
         }
         __syncwarp();
-        if (ok) {
-          uint8_t *dst = smem + (size_t)stage * S::kStageBytes + is_v * S::kTileBytes + blk * kBlkBytes +
-                         box * box_bytes;
-          const CUtensorMap *tm = is_v ? &tm_v : &tm_k;
-          tma_load_4d(dst, tm, blk * 64, key % A.pt.page_size, hk, page, &full[stage]);
-        }
+        if (ok)
+          tma_load_4d(smem + (size_t)stage * C::kStageBytes + is_v * C::kTileBytes + blk * kBlkBytes + box * box_bytes,
+                      is_v ? &tm_v : &tm_k, blk * 64, key % A.pt.page_size, hk, page, &full[stage]);
         page = page_next;
         key = key_next;
         seen = seen_next;
@@ -394,18 +440,19 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
     // CTA's memory when it exits
     __syncwarp();
     if (*(volatile int *)&aborted && lane == 0)
-      for (int i = 0; i < A.stages; i++) {
+      for (int i = 0; i < S; i++) {
         mbar_wait_bounded(&full[stage], phase ^ 1, A.flags);
         advance();
       }
   } else {
     // ---- consumers ----
+    const int wk = warp & 3, wr = warp >> 2;  // this warp's keys and rows
     const int g = lane >> 2, t4 = lane & 3;
     const int jm = lane >> 3, jr = lane & 7;  // ldmatrix: this lane addresses row jr of matrix jm
     int rec_parts = 0;
-    int rec[6] = {0, 0, 0, 0, 0, 0};
+    int rec[5] = {0, 0, 0, 0, 0};
     for (int pos = start; pos < end;) {
-      const SeqWork w = seq_work(A, b, S::kRows);
+      const SeqWork w = seq_work(A, b, C::kRows, kKeys);
       const int work = A.Hkv * w.mt * w.nt;
       if (pos >= base + work) {
         base += work;
@@ -414,58 +461,66 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
       }
       const int unit = (pos - base) / w.nt, t0 = (pos - base) - unit * w.nt;
       const int t1 = min(w.nt, t0 + (end - pos));
-      const int hk = unit / w.mt, m0 = (unit - hk * w.mt) * S::kRows;
+      const int hk = unit / w.mt, m0 = (unit - hk * w.mt) * C::kRows;
 
-      // queries as A fragments; the position of each of this thread's rows
-      uint32_t qa[MT][Dh / 16][4];
-      int rp[MT][2];
-#pragma unroll
-      for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int m = m0 + mt * 16 + g + 8 * e, i = m / A.G;
-          const bool valid = i < w.n;
-          const long long rpos = valid ? (long long)w.p + i : -1;
-          rp[mt][e] = (int)max(-1LL, min(rpos, 0x7ffffffeLL));
-          const T *src = reinterpret_cast<const T *>(A.q) +
-                         ((size_t)(w.r0 + (valid ? i : 0)) * A.H + hk * A.G + (valid ? m - i * A.G : 0)) * Dh + 2 * t4;
-#pragma unroll
-          for (int kk = 0; kk < Dh / 16; kk++) {
-            qa[mt][kk][e] = valid ? *reinterpret_cast<const uint32_t *>(src + 16 * kk) : 0u;
-            qa[mt][kk][e + 2] = valid ? *reinterpret_cast<const uint32_t *>(src + 16 * kk + 8) : 0u;
-          }
-        }
-      float o[MT][Dh / 8][4];
-      float mx[MT][2], ls[MT][2];
-#pragma unroll
-      for (int mt = 0; mt < MT; mt++) {
-        mx[mt][0] = mx[mt][1] = -INFINITY;
-        ls[mt][0] = ls[mt][1] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < Dh / 8; d++) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.0f;
+      // queries, 16 bytes a load, through the merge buffer into A fragments; the
+      // position of each of this thread's rows
+      auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(C::kWarps * 32) : "memory"); };
+      T *sq = reinterpret_cast<T *>(red);
+      constexpr int kQRow = Dh + 8;
+      for (int i = tid; i < C::kRows * (Dh / 8); i += C::kWarps * 32) {
+        const int row = i / (Dh / 8), ch = i - row * (Dh / 8), m = m0 + row, qi = m / A.G;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (qi < w.n)
+          v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(A.q) +
+                                                    ((size_t)(w.r0 + qi) * A.H + hk * A.G + (m - qi * A.G)) * Dh) +
+                    ch);
+        *reinterpret_cast<uint4 *>(sq + row * kQRow + ch * 8) = v;
       }
+      int rp[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int i = (m0 + wr * 16 + g + 8 * e) / A.G;
+        rp[e] = (int)max(-1LL, min(i < w.n ? (long long)w.p + i : -1LL, 0x7ffffffeLL));
+      }
+      sync();
+      uint32_t qa[Dh / 16][4];
+#pragma unroll
+      for (int kk = 0; kk < Dh / 16; kk++)
+        ldsm4(smem_u32(sq + (wr * 16 + (jm & 1) * 8 + jr) * kQRow + kk * 16 + (jm >> 1) * 8), qa[kk]);
+      sync();  // the buffer is free again
+      float o[Dh / 8][4];
+      float mx[2] = {-INFINITY, -INFINITY}, ls[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int d = 0; d < Dh / 8; d++) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
       const long long p_last = (long long)w.p + w.n - 1;
 
       for (int t = t0; t < t1; t++) {
         wait(&full[stage], phase);
-        const int key0 = (t < w.a ? t : t - w.a + w.c) * kKeys + warp * 16;  // this warp's 16 keys
-        const bool have = held[stage] >> (warp * 16 / A.box_rows) & 1;
+        const int key0 = (t < w.a ? t : t - w.a + w.c) * kKeys + wk * KW;  // this warp's keys
+        constexpr int kAll = (1 << (KW / 16)) - 1;
+        const int have = held[stage] >> (wk * KW / 16) & kAll;
         if (have) {
-          const uint32_t kaddr = smem_u32(smem) + (uint32_t)stage * S::kStageBytes;
-          const uint32_t vaddr = kaddr + S::kTileBytes;
-          // every row sees every one of the 16 keys
-          const bool open = key0 + 15 <= w.p &&
-                            (A.window == 0 || key0 + 15 < A.sinks || (long long)key0 > p_last - A.window);
+          uint8_t *stage_v = smem + (size_t)stage * C::kStageBytes + C::kTileBytes;
+          const uint32_t kaddr = smem_u32(smem) + (uint32_t)stage * C::kStageBytes;
+          const uint32_t vaddr = kaddr + C::kTileBytes;
+          // every row sees every one of the keys
+          const bool open = key0 + KW - 1 <= w.p && have == kAll &&
+                            (A.window == 0 || key0 + KW - 1 < A.sinks || (long long)key0 > p_last - A.window);
+          // whether some row of the sequence sees key i of these
+          auto seen = [&](int i) {
+            const int key = key0 + i;
+            return key < w.hi && (key < w.se || key >= w.ws) && (have >> (i >> 4) & 1);
+          };
           bool odd = false;  // some V row that not every row sees holds an infinity or NaN
           if (!open) {
             // V rows that no row of the sequence sees: zeros (their P is 0,
             // and 0 times whatever the page holds there would not be)
-            for (int i = lane; i < 16 * (Dh / 8); i += 32) {
-              const int kr = i / (Dh / 8), ch = i - kr * (Dh / 8), key = key0 + kr, row = warp * 16 + kr;
-              uint8_t *at = smem + (size_t)stage * S::kStageBytes + S::kTileBytes + (ch >> 3) * kBlkBytes +
-                            row * 128 + (((ch & 7) ^ (row & 7)) << 4);
-              uint4 *v = reinterpret_cast<uint4 *>(at);
-              if (key >= w.hi || (key >= w.se && key < w.ws)) {
+            for (int i = lane; i < KW * (Dh / 8); i += 32) {
+              const int kr = i / (Dh / 8), ch = i - kr * (Dh / 8), row = wk * KW + kr;
+              uint4 *v = reinterpret_cast<uint4 *>(stage_v + (ch >> 3) * kBlkBytes + row * 128 +
+                                                   (((ch & 7) ^ (row & 7)) << 4));
+              if (!seen(kr)) {
                 *v = make_uint4(0, 0, 0, 0);
               } else {
                 const uint4 u = *v;
@@ -476,127 +531,120 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
             __syncwarp();  // the zeros, before the reads below
           }
           // S = Q K^T
-          float s[MT][2][4];
+          float s[KW / 8][4];
 #pragma unroll
-          for (int mt = 0; mt < MT; mt++)
+          for (int nt = 0; nt < KW / 8; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
-          {
-            const int row = warp * 16 + 8 * (jm >> 1) + jr;
+          for (int kk = 0; kk < Dh / 16; kk++) {
+            const int ch = 2 * kk + (jm & 1);
 #pragma unroll
-            for (int kk = 0; kk < Dh / 16; kk++) {
-              const int ch = 2 * kk + (jm & 1);
+            for (int np = 0; np < KW / 16; np++) {
+              const int row = wk * KW + np * 16 + 8 * (jm >> 1) + jr;
               uint32_t bf[4];
               ldsm4(kaddr + (ch >> 3) * kBlkBytes + row * 128 + (((ch & 7) ^ (row & 7)) << 4), bf);
-#pragma unroll
-              for (int mt = 0; mt < MT; mt++) {
-                mma16816<T>(s[mt][0], qa[mt][kk], bf[0], bf[1]);
-                mma16816<T>(s[mt][1], qa[mt][kk], bf[2], bf[3]);
-              }
+              mma16816<T>(s[2 * np], qa[kk], bf[0], bf[1]);
+              mma16816<T>(s[2 * np + 1], qa[kk], bf[2], bf[3]);
             }
           }
           if (!open) {
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int nt = 0; nt < KW / 8; nt++)
 #pragma unroll
-              for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                  const int key = key0 + nt * 8 + 2 * t4 + (e & 1), p = rp[mt][e >> 1];
-                  if (key >= w.hi || !sees_key(p, key, A.window, A.sinks)) s[mt][nt][e] = -INFINITY;
-                }
-          }
-          // online softmax; the probabilities as hi + lo halves
-          uint32_t ph[MT][4], pl[MT][4];
-#pragma unroll
-          for (int mt = 0; mt < MT; mt++) {
-            float f[2];
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              float m = fmaxf(fmaxf(s[mt][0][2 * e], s[mt][0][2 * e + 1]), fmaxf(s[mt][1][2 * e], s[mt][1][2 * e + 1]));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-              const float mn = fmaxf(mx[mt][e], m * kLog2e);
-              f[e] = mn == -INFINITY ? 1.0f : ex2(mx[mt][e] - mn);
-              const float sub = mn == -INFINITY ? 0.0f : mn;
-              mx[mt][e] = mn;
-              float sum = 0.0f;
-#pragma unroll
-              for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                  const float v = ex2(s[mt][nt][2 * e + c] * kLog2e - sub);
-                  s[mt][nt][2 * e + c] = v;
-                  sum += v;
-                }
-              ls[mt][e] = ls[mt][e] * f[e] + sum;
-            }
-            if (f[0] != 1.0f || f[1] != 1.0f) {
-#pragma unroll
-              for (int d = 0; d < Dh / 8; d++) {
-                o[mt][d][0] *= f[0];
-                o[mt][d][1] *= f[0];
-                o[mt][d][2] *= f[1];
-                o[mt][d][3] *= f[1];
+              for (int e = 0; e < 4; e++) {
+                const int i = nt * 8 + 2 * t4 + (e & 1);
+                if (!seen(i) || !sees_key(rp[e >> 1], key0 + i, A.window, A.sinks)) s[nt][e] = -INFINITY;
               }
-            }
+          }
+          // online softmax
+          float f[2];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const float v0 = s[mt][i >> 1][2 * (i & 1)], v1 = s[mt][i >> 1][2 * (i & 1) + 1];
-              ph[mt][i] = pack2<T>(v0, v1);
-              const float2 h = unpack2<T>(ph[mt][i]);
-              pl[mt][i] = pack2<T>(v0 - h.x, v1 - h.y);
+          for (int e = 0; e < 2; e++) {
+            float m = fmaxf(s[0][2 * e], s[0][2 * e + 1]);
+#pragma unroll
+            for (int nt = 1; nt < KW / 8; nt++) m = fmaxf(m, fmaxf(s[nt][2 * e], s[nt][2 * e + 1]));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const float mn = fmaxf(mx[e], m * kLog2e);
+            f[e] = mn == -INFINITY ? 1.0f : ex2(mx[e] - mn);
+            const float sub = mn == -INFINITY ? 0.0f : mn;
+            mx[e] = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int nt = 0; nt < KW / 8; nt++)
+#pragma unroll
+              for (int c = 0; c < 2; c++) {
+                const float v = ex2(s[nt][2 * e + c] * kLog2e - sub);
+                s[nt][2 * e + c] = v;
+                sum += v;
+              }
+            ls[e] = ls[e] * f[e] + sum;
+          }
+          if (f[0] != 1.0f || f[1] != 1.0f) {
+#pragma unroll
+            for (int d = 0; d < Dh / 8; d++) {
+              o[d][0] *= f[0];
+              o[d][1] *= f[0];
+              o[d][2] *= f[1];
+              o[d][3] *= f[1];
             }
           }
           // O += P V
           if (!odd) {
-            const int row = warp * 16 + 8 * (jm & 1) + jr;
 #pragma unroll
-            for (int dp = 0; dp < Dh / 16; dp++) {
-              const int ch = 2 * dp + (jm >> 1);
-              uint32_t bf[4];
-              ldsm4_t(vaddr + (ch >> 3) * kBlkBytes + row * 128 + (((ch & 7) ^ (row & 7)) << 4), bf);
+            for (int kc = 0; kc < KW / 16; kc++) {
+              uint32_t ph[4], pl[4];  // P of 16 keys as hi + lo halves
 #pragma unroll
-              for (int mt = 0; mt < MT; mt++) {
-                mma16816<T>(o[mt][2 * dp], ph[mt], bf[0], bf[1]);
-                mma16816<T>(o[mt][2 * dp], pl[mt], bf[0], bf[1]);
-                mma16816<T>(o[mt][2 * dp + 1], ph[mt], bf[2], bf[3]);
-                mma16816<T>(o[mt][2 * dp + 1], pl[mt], bf[2], bf[3]);
+              for (int i = 0; i < 4; i++) {
+                const float v0 = s[2 * kc + (i >> 1)][2 * (i & 1)], v1 = s[2 * kc + (i >> 1)][2 * (i & 1) + 1];
+                ph[i] = pack2<T>(v0, v1);
+                const float2 h = unpack2<T>(ph[i]);
+                pl[i] = pack2<T>(v0 - h.x, v1 - h.y);
+              }
+              const int row = wk * KW + kc * 16 + 8 * (jm & 1) + jr;
+#pragma unroll
+              for (int dp = 0; dp < Dh / 16; dp++) {
+                const int ch = 2 * dp + (jm >> 1);
+                uint32_t bf[4];
+                ldsm4_t(vaddr + (ch >> 3) * kBlkBytes + row * 128 + (((ch & 7) ^ (row & 7)) << 4), bf);
+                mma16816<T>(o[2 * dp], ph, bf[0], bf[1]);
+                mma16816<T>(o[2 * dp + 1], ph, bf[2], bf[3]);
+                mma16816<T>(o[2 * dp], pl, bf[0], bf[1]);
+                mma16816<T>(o[2 * dp + 1], pl, bf[2], bf[3]);
               }
             }
           } else {
-            // one key at a time, for the rows that see it
-            for (int kr = 0; kr < 16; kr++) {
-              const int key = key0 + kr, row = warp * 16 + kr, src = (lane & ~3) | ((kr & 7) >> 1);
+            // one key at a time, for the rows that see it (rare: kept small)
+            float *sp = red + warp * 16 * KW;
 #pragma unroll
-              for (int mt = 0; mt < MT; mt++) {
-                float pv[2];
-                bool see[2];
+            for (int nt = 0; nt < KW / 8; nt++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                  const float lo = kr < 8 ? s[mt][0][2 * e] : s[mt][1][2 * e];
-                  const float hi = kr < 8 ? s[mt][0][2 * e + 1] : s[mt][1][2 * e + 1];
-                  pv[e] = __shfl_sync(0xffffffffu, kr & 1 ? hi : lo, src);
-                  const int p = rp[mt][e];
-                  see[e] = key < w.hi && sees_key(p, key, A.window, A.sinks);
+              for (int e = 0; e < 4; e++) sp[(g + 8 * (e >> 1)) * KW + nt * 8 + 2 * t4 + (e & 1)] = s[nt][e];
+            __syncwarp();
+#pragma unroll 1
+            for (int kr = 0; kr < KW; kr++) {
+              const int row = wk * KW + kr;
+              float pv[2];
+              bool see[2];
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                pv[e] = sp[(g + 8 * e) * KW + kr];
+                see[e] = seen(kr) && sees_key(rp[e], key0 + kr, A.window, A.sinks);
+              }
+#pragma unroll
+              for (int d = 0; d < Dh / 8; d++) {
+                const float2 v = unpack2<T>(*reinterpret_cast<const uint32_t *>(
+                    stage_v + (d >> 3) * kBlkBytes + row * 128 + (((d & 7) ^ (row & 7)) << 4) + 4 * t4));
+                if (see[0]) {
+                  o[d][0] += pv[0] * v.x;
+                  o[d][1] += pv[0] * v.y;
                 }
-#pragma unroll
-                for (int d = 0; d < Dh / 8; d++) {
-                  const uint32_t u = *reinterpret_cast<const uint32_t *>(
-                      smem + (size_t)stage * S::kStageBytes + S::kTileBytes + (d >> 3) * kBlkBytes + row * 128 +
-                      (((d & 7) ^ (row & 7)) << 4) + 4 * t4);
-                  const float2 v = unpack2<T>(u);
-                  if (see[0]) {
-                    o[mt][d][0] += pv[0] * v.x;
-                    o[mt][d][1] += pv[0] * v.y;
-                  }
-                  if (see[1]) {
-                    o[mt][d][2] += pv[1] * v.x;
-                    o[mt][d][3] += pv[1] * v.y;
-                  }
+                if (see[1]) {
+                  o[d][2] += pv[1] * v.x;
+                  o[d][3] += pv[1] * v.y;
                 }
               }
             }
+            __syncwarp();
           }
           if (!open) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the zeros, before the next copy
         }
@@ -606,77 +654,68 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
       }
 
       // ---- the warps' shares together ----
-      auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kSplitWarps * 32) : "memory"); };
 #pragma unroll
-      for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          float l = ls[mt][e];
-          l += __shfl_xor_sync(0xffffffffu, l, 1);
-          l += __shfl_xor_sync(0xffffffffu, l, 2);
-          if (t4 == 0) {
-            sm_m[warp * S::kRows + mt * 16 + g + 8 * e] = mx[mt][e];
-            sm_l[warp * S::kRows + mt * 16 + g + 8 * e] = l;
-          }
+      for (int e = 0; e < 2; e++) {
+        float l = ls[e];
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t4 == 0) {
+          sm_m[wk * C::kRows + wr * 16 + g + 8 * e] = mx[e];
+          sm_l[wk * C::kRows + wr * 16 + g + 8 * e] = l;
         }
+      }
       sync();
 #pragma unroll
-      for (int mt = 0; mt < MT; mt++)
+      for (int e = 0; e < 2; e++) {
+        const int row = wr * 16 + g + 8 * e;
+        float m = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int row = mt * 16 + g + 8 * e;
-          float m = -INFINITY;
+        for (int i = 0; i < 4; i++) m = fmaxf(m, sm_m[i * C::kRows + row]);
+        const float f = m == -INFINITY ? 0.0f : ex2(mx[e] - m);
 #pragma unroll
-          for (int i = 0; i < kSplitWarps; i++) m = fmaxf(m, sm_m[i * S::kRows + row]);
-          const float f = m == -INFINITY ? 0.0f : ex2(mx[mt][e] - m);
-#pragma unroll
-          for (int d = 0; d < Dh / 8; d++) {
-            o[mt][d][2 * e] *= f;
-            o[mt][d][2 * e + 1] *= f;
-          }
+        for (int d = 0; d < Dh / 8; d++) {
+          o[d][2 * e] *= f;
+          o[d][2 * e + 1] *= f;
         }
-      auto put = [&](float *dst) {
+      }
+      // key groups 2 and 3 leave their sums, 0 and 1 add theirs
+      float *mine = red + ((wk & 1) * C::kRows + wr * 16) * C::kRedRow;
+      if (wk >= 2) {
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int d = 0; d < Dh / 8; d++)
 #pragma unroll
-          for (int d = 0; d < Dh / 8; d++)
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-              *reinterpret_cast<float2 *>(dst + (mt * 16 + g + 8 * e) * Dh + d * 8 + 2 * t4) =
-                  make_float2(o[mt][d][2 * e], o[mt][d][2 * e + 1]);
-      };
-      if (warp >= 2) put(red + (warp - 2) * S::kRows * Dh);
+          for (int e = 0; e < 2; e++)
+            *reinterpret_cast<float2 *>(mine + (g + 8 * e) * C::kRedRow + d * 8 + 2 * t4) =
+                make_float2(o[d][2 * e], o[d][2 * e + 1]);
+      }
       sync();
-      if (warp < 2) {
-        float *mine = red + warp * S::kRows * Dh;
+      if (wk < 2) {
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int d = 0; d < Dh / 8; d++)
 #pragma unroll
-          for (int d = 0; d < Dh / 8; d++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              float2 *at = reinterpret_cast<float2 *>(mine + (mt * 16 + g + 8 * e) * Dh + d * 8 + 2 * t4);
-              float2 v = *at;
-              v.x += o[mt][d][2 * e];
-              v.y += o[mt][d][2 * e + 1];
-              *at = v;
-            }
+          for (int e = 0; e < 2; e++) {
+            float2 *at = reinterpret_cast<float2 *>(mine + (g + 8 * e) * C::kRedRow + d * 8 + 2 * t4);
+            float2 v = *at;
+            v.x += o[d][2 * e];
+            v.y += o[d][2 * e + 1];
+            *at = v;
+          }
       }
       sync();
       const bool whole = t0 == 0 && t1 == w.nt;
       const int slot = 2 * cta + (pos == start ? 0 : 1);
-      float *part = A.part + (size_t)slot * S::kRows * (Dh + 2);
-      for (int i = tid; i < S::kRows * (Dh / 4); i += kSplitWarps * 32) {
+      float *part = A.part + (size_t)slot * C::kRows * (Dh + 2);
+      for (int i = tid; i < C::kRows * (Dh / 4); i += C::kWarps * 32) {
         const int row = i / (Dh / 4), d = (i - row * (Dh / 4)) * 4, m = m0 + row, qi = m / A.G;
         if (qi >= w.n) continue;
         float mm = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kSplitWarps; k++) mm = fmaxf(mm, sm_m[k * S::kRows + row]);
+        for (int k = 0; k < 4; k++) mm = fmaxf(mm, sm_m[k * C::kRows + row]);
 #pragma unroll
-        for (int k = 0; k < kSplitWarps; k++)
-          l += mm == -INFINITY ? 0.0f : sm_l[k * S::kRows + row] * ex2(sm_m[k * S::kRows + row] - mm);
-        const float4 x = *reinterpret_cast<const float4 *>(red + row * Dh + d);
-        const float4 y = *reinterpret_cast<const float4 *>(red + (S::kRows + row) * Dh + d);
+        for (int k = 0; k < 4; k++)
+          l += mm == -INFINITY ? 0.0f : sm_l[k * C::kRows + row] * ex2(sm_m[k * C::kRows + row] - mm);
+        const float4 x = *reinterpret_cast<const float4 *>(red + row * C::kRedRow + d);
+        const float4 y = *reinterpret_cast<const float4 *>(red + (C::kRows + row) * C::kRedRow + d);
         float4 v = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
         if (whole) {
           const float inv = mm == -INFINITY ? 0.0f : 1.0f / l;
@@ -686,10 +725,10 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 && Dh <= 128 ? 2 : 1)
           *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(A.out) +
                                      ((size_t)(w.r0 + qi) * A.H + hk * A.G + (m - qi * A.G)) * Dh + d) = u;
         } else {
-          *reinterpret_cast<float4 *>(part + 2 * S::kRows + row * Dh + d) = v;
+          *reinterpret_cast<float4 *>(part + 2 * C::kRows + row * Dh + d) = v;
           if (d == 0) {
             part[row] = mm;
-            part[S::kRows + row] = l;
+            part[C::kRows + row] = l;
           }
         }
       }
@@ -803,34 +842,31 @@ cudaError_t rope_t(const float *qkv, const PagedRows &pr, int H, int Hkv, const 
                 hpw, wpr, flags);
 }
 
-constexpr int split_ctas_per_sm(int Dh, int MT) { return MT == 1 && Dh <= 128 ? 2 : 1; }
-constexpr int kSplitSmemPerSm = 224 * 1024;
-
 template <typename T, int Dh, int MT>
 cudaError_t split_t(SplitArgs A, const wg_paged_kv &kv, void *workspace, int num_sms, cudaStream_t s, bool pdl) {
-  using S = SplitSmem<T, Dh, MT>;
-  const int occ = split_ctas_per_sm(Dh, MT);
-  const int budget = kSplitSmemPerSm / occ - 1024;
-  A.stages = (budget - S::kFixed) / S::kStageBytes;
-  if (A.stages > kMaxStages) A.stages = kMaxStages;
-  static_assert((kSplitSmemPerSm / split_ctas_per_sm(Dh, MT) - 1024 - S::kFixed) / S::kStageBytes >= 2, "two stages");
-  const size_t smem = (size_t)A.stages * S::kStageBytes + S::kFixed;
+  using C = SplitCfg<Dh, MT>;
   auto kern = paged_split_kernel<T, Dh, MT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return e;
+  // keys of a box: the largest power of two that divides the page, up to 64
+  A.box_rows = kv.page_size % 64 == 0 ? 64 : kv.page_size % 32 == 0 ? 32 : 16;
   CUtensorMap tk, tv;
   if (!page_map(&tk, kv.k, kv, A.Hkv, Dh, A.box_rows) || !page_map(&tv, kv.v, kv, A.Hkv, Dh, A.box_rows))
     return cudaErrorInvalidValue;
-  const int P = num_sms * occ;
+  // CTAs: no more than there can be work for
+  const long long units = (((long long)A.pr.rows * A.G + C::kRows - 1) / C::kRows + A.pr.batch) * A.Hkv;
+  const long long keys = (long long)kv.max_pages * kv.page_size;
+  const long long work = units * ((keys + kMinKeys - 1) / kMinKeys);
+  const int P = (int)(work < num_sms * C::kCtas ? work : num_sms * C::kCtas);
   A.rec = reinterpret_cast<int *>(workspace);
   A.part = reinterpret_cast<float *>(A.rec + (size_t)P * 8);
-  e = launch_pdl(kern, dim3((unsigned)P), kSplitThreads, smem, s, pdl, tk, tv, A);
+  e = launch_pdl(kern, dim3((unsigned)P), C::kThreads, C::kSmem, s, pdl, tk, tv, A);
   if (e != cudaSuccess) return e;
   // rows of a unit that can exist: none past the longest sequence's
   const long long most = A.pr.row_start ? A.pr.rows : A.pr.rows / A.pr.batch;
-  const unsigned rows = (unsigned)(most * A.G < S::kRows ? most * A.G : S::kRows);
-  return launch_pdl(paged_join_kernel<T, Dh>, dim3((unsigned)P, rows), kJoinThreads, 0, s, pdl, A.rec, A.part, S::kRows,
-                A.H, A.G, reinterpret_cast<T *>(A.out));
+  const unsigned rows = (unsigned)(most * A.G < C::kRows ? most * A.G : C::kRows);
+  return launch_pdl(paged_join_kernel<T, Dh>, dim3((unsigned)P, rows), kJoinThreads, 0, s, pdl, A.rec, A.part,
+                    C::kRows, A.H, A.G, reinterpret_cast<T *>(A.out));
 }
 
 template <typename T>
@@ -875,14 +911,10 @@ cudaError_t launch_paged_rope_kv(const float *qkv, const PagedRows &rows, int H,
 }
 
 size_t paged_attention_workspace(int Dh, int num_sms) {
-  // the larger of the 16-row and the 32-row kernels' needs
-  size_t most = 0;
-  for (int mt = 1; mt <= 2; mt++) {
-    const size_t P = (size_t)num_sms * split_ctas_per_sm(Dh, mt);
-    const size_t need = P * 8 * sizeof(int) + 2 * P * (16 * mt) * (size_t)(Dh + 2) * sizeof(float);
-    if (need > most) most = need;
-  }
-  return most;
+  // the larger of the 16-row (two CTAs an SM, but for Dh = 256) and the 32-row
+  // kernels' needs: the same number of rows in all
+  const size_t P = (size_t)num_sms * 2;
+  return P * 8 * sizeof(int) + 2 * P * 16 * (size_t)(Dh + 2) * sizeof(float);
 }
 
 cudaError_t launch_paged_attention(const void *q, const PagedRows &rows, int H, int Hkv, int Dh,
@@ -900,7 +932,6 @@ cudaError_t launch_paged_attention(const void *q, const PagedRows &rows, int H, 
   A.G = H / Hkv;
   A.window = window;
   A.sinks = sinks;
-  A.box_rows = kv.page_size % 64 == 0 ? 64 : kv.page_size % 32 == 0 ? 32 : 16;
   A.flags = flags;
   return kv.dtype == WG_F16 ? split_d<__half>(A, Dh, kv, workspace, num_sms, s, pdl)
                             : split_d<__nv_bfloat16>(A, Dh, kv, workspace, num_sms, s, pdl);

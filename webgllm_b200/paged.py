@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import WG_BF16, WG_F16, GpuError, ShapeError, wg_paged_kv
-from .q4 import Context, context
+from .q4 import context
 
 __all__ = ["attention_paged", "rope_kv_paged"]
 
@@ -36,44 +36,36 @@ def _arg(msg: str):
     return GpuError(_lib.WG_INVALID_ARGUMENT, msg)
 
 
-def _int32(t: torch.Tensor, what: str, shape: tuple, device) -> int:
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
-        raise _arg(f"{what} must be a contiguous int32 {list(shape)} tensor on {device}")
+def _int32(t: torch.Tensor, what: str, shape: tuple, device: int) -> int:
+    if t.dtype is not torch.int32 or t.get_device() != device or t.shape != shape or not t.is_contiguous():
+        raise _arg(f"{what} must be a contiguous int32 {list(shape)} tensor on CUDA device {device}")
     return t.data_ptr()
 
 
-def _cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, batch: int) -> wg_paged_kv:
-    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride():
-        raise _bad(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [pages][KV heads][page size][head dim] alike")
+def _check_out(t: torch.Tensor, dtype, shape: tuple, device: int) -> None:
+    if t.dtype is not dtype or t.get_device() != device or t.shape != shape or not t.is_contiguous():
+        raise _arg(f"out must be a contiguous {dtype} {list(shape)} tensor on CUDA device {device}")
+
+
+def _cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, batch: int, device: int) -> wg_paged_kv:
+    shape, strides = k.shape, k.stride()
+    if len(shape) != 4 or v.shape != shape or v.stride() != strides:
+        raise _bad(f"k {tuple(shape)} and v {tuple(v.shape)} must be [pages][KV heads][page size][head dim] alike")
     code = _CODES.get(k.dtype)
-    if code is None or v.dtype != k.dtype:
+    if code is None or v.dtype is not k.dtype:
         raise _arg(f"pages must be float16 or bfloat16, not {k.dtype} and {v.dtype}")
-    if not k.is_cuda or v.device != k.device:
+    if device < 0 or v.get_device() != device:
         raise _arg("pages must be CUDA tensors of one device")
     if table.dim() != 2 or table.shape[0] != batch:
         raise _bad(f"table {tuple(table.shape)} must be [{batch}][pages of a sequence]")
-    t = _int32(table, "table", tuple(table.shape), k.device)
-    pages, _, size, dim = k.shape
-    # the stride of a dimension of one entry is never walked and may be anything
-    sp, sh, sr, sd = (0 if n == 1 else s for n, s in zip(k.shape, k.stride()))
-    if sd not in (0, 1) or (sp | sh | sr) % 8 or any(n > 1 and s <= 0 for n, s in zip(k.shape[:3], (sp, sh, sr))):
-        raise _bad(f"pages of strides {k.stride()}: the last must be 1, the others positive multiples of 8")
-    return wg_paged_kv(k.data_ptr(), v.data_ptr(), t, code, pages, size, table.shape[1], sp, sh, sr)
-
-
-def _context(device: torch.device) -> Context:
-    ctx = context(device.index)
-    ctx.use_torch_stream()
-    return ctx
-
-
-def _call(ctx: Context, fn, *args) -> None:
-    """fn(ctx, *args) with the caller's current device left as it was."""
-    if torch.cuda.current_device() == ctx.device:
-        ctx._check(fn(ctx.handle, *args))
-    else:
-        with torch.cuda.device(ctx.device):
-            ctx._check(fn(ctx.handle, *args))
+    t = _int32(table, "table", table.shape, device)
+    sp, sh, sr, sd = strides
+    if sd != 1 or (sp | sh | sr) & 7 or sp <= 0 or sh <= 0 or sr <= 0:
+        # the stride of a dimension of one entry is never walked and may be anything
+        sp, sh, sr, sd = (0 if n == 1 else s for n, s in zip(shape, strides))
+        if sd > 1 or (sp | sh | sr) & 7 or any(n > 1 and s <= 0 for n, s in zip(shape, (sp, sh, sr, sd))):
+            raise _bad(f"pages of strides {strides}: the last must be 1, the others positive multiples of 8")
+    return wg_paged_kv(k.data_ptr(), v.data_ptr(), t, code, shape[0], shape[2], table.shape[1], sp, sh, sr)
 
 
 def _ptr(t: torch.Tensor | None):
@@ -89,41 +81,39 @@ def rope_kv_paged(qkv: torch.Tensor, pos: torch.Tensor, k: torch.Tensor, v: torc
     scaled queries [rows][heads][head dim] in the pages' dtype; keys and values
     go into the pages. Rows that belong to no sequence stay as they were in
     `out` (uninitialised in a new one)."""
-    batch = pos.numel()
-    kv = _cache(k, v, table, batch)
-    hkv, dim, device = k.shape[1], k.shape[3], k.device
+    batch, device = pos.numel(), k.get_device()
+    kv = _cache(k, v, table, batch, device)
+    _, hkv, _, dim = k.shape
     if qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * hkv) * dim:
         raise _bad(f"qkv {tuple(qkv.shape)} does not hold {heads} + 2 x {hkv} heads of {dim}")
-    if qkv.dtype != torch.float32 or qkv.device != device:
-        raise _arg(f"qkv must be float32 on {device}")
+    if qkv.dtype is not torch.float32 or qkv.get_device() != device:
+        raise _arg(f"qkv must be float32 on CUDA device {device}")
     if not qkv.is_contiguous():
         qkv = qkv.contiguous()
     rows = qkv.shape[0]
     for n in (q_norm, k_norm):
-        if n is not None and (n.dtype != torch.float32 or n.device != device or n.shape != (dim,)
+        if n is not None and (n.dtype is not torch.float32 or n.get_device() != device or n.shape != (dim,)
                               or not n.is_contiguous()):
-            raise _arg(f"norm weights must be contiguous float32 [{dim}] on {device}")
+            raise _arg(f"norm weights must be contiguous float32 [{dim}] on CUDA device {device}")
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=k.dtype, device=device)
-    elif out.shape != (rows, heads, dim) or out.dtype != k.dtype or out.device != device or not out.is_contiguous():
-        raise _arg(f"out must be a contiguous {k.dtype} [{rows}][{heads}][{dim}] tensor on {device}")
+        out = torch.empty((rows, heads, dim), dtype=k.dtype, device=k.device)
+    else:
+        _check_out(out, k.dtype, (rows, heads, dim), device)
     p = _int32(pos, "pos", (batch,), device)
     rs = None if row_start is None else _int32(row_start, "row_start", (batch + 1,), device)
-    ctx = _context(device)
-    _call(ctx, _lib.lib().wg_paged_rope_kv, qkv.data_ptr(), rows, batch, rs, heads, hkv, dim, p, theta, _ptr(q_norm),
-          _ptr(k_norm), eps, out.data_ptr(), ctypes.byref(kv))
+    context(device).enqueue(_lib.lib().wg_paged_rope_kv, qkv.data_ptr(), rows, batch, rs, heads, hkv, dim, p, theta,
+                            _ptr(q_norm), _ptr(k_norm), eps, out.data_ptr(), ctypes.byref(kv))
     return out
 
 
-def workspace_bytes(device: torch.device, head_dim: int) -> int:
-    """wg_paged_attention_workspace."""
-    key = (device.index, head_dim)
-    n = _workspace_bytes.get(key)
+def workspace_bytes(device: int, head_dim: int) -> int:
+    """wg_paged_attention_workspace on a CUDA device (its index)."""
+    n = _workspace_bytes.get((device, head_dim))
     if n is None:
         b = ctypes.c_size_t()
-        ctx = context(device.index)
+        ctx = context(device)
         ctx._check(_lib.lib().wg_paged_attention_workspace(ctx.handle, head_dim, ctypes.byref(b)))
-        n = _workspace_bytes[key] = b.value
+        n = _workspace_bytes[device, head_dim] = b.value
     return n
 
 
@@ -136,27 +126,26 @@ def attention_paged(q: torch.Tensor, pos: torch.Tensor, k: torch.Tensor, v: torc
     and the first `sinks` positions. `workspace`: a uint8 tensor of
     workspace_bytes(...) that no overlapping call uses (default: a new one from
     torch's allocator, safe on any stream and inside a graph)."""
-    batch = pos.numel()
-    kv = _cache(k, v, table, batch)
-    hkv, dim, device = k.shape[1], k.shape[3], k.device
+    batch, device = pos.numel(), k.get_device()
+    kv = _cache(k, v, table, batch, device)
+    _, hkv, _, dim = k.shape
     if q.dim() != 3 or q.shape[2] != dim or q.shape[1] % hkv:
         raise _bad(f"q {tuple(q.shape)} does not match {hkv} KV heads of {dim}")
-    if q.dtype != k.dtype or q.device != device:
-        raise _arg(f"q must be {k.dtype} on {device}")
+    if q.dtype is not k.dtype or q.get_device() != device:
+        raise _arg(f"q must be {k.dtype} on CUDA device {device}")
     if not q.is_contiguous():
         q = q.contiguous()
-    rows, heads = q.shape[0], q.shape[1]
+    rows, heads, _ = q.shape
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous():
-        raise _arg(f"out must be a contiguous {q.dtype} {list(q.shape)} tensor on {device}")
+    else:
+        _check_out(out, q.dtype, q.shape, device)
     p = _int32(pos, "pos", (batch,), device)
     rs = None if row_start is None else _int32(row_start, "row_start", (batch + 1,), device)
-    ctx = _context(device)
     if workspace is None:
-        workspace = torch.empty(workspace_bytes(device, dim), dtype=torch.uint8, device=device)
-    elif workspace.device != device or not workspace.is_contiguous():
-        raise _arg(f"workspace must be contiguous on {device}")
-    _call(ctx, _lib.lib().wg_paged_attention, q.data_ptr(), rows, batch, rs, heads, hkv, dim, p, ctypes.byref(kv),
-          window, sinks, out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        workspace = torch.empty(workspace_bytes(device, dim), dtype=torch.uint8, device=k.device)
+    elif workspace.get_device() != device or not workspace.is_contiguous():
+        raise _arg(f"workspace must be contiguous on CUDA device {device}")
+    context(device).enqueue(_lib.lib().wg_paged_attention, q.data_ptr(), rows, batch, rs, heads, hkv, dim, p,
+                            ctypes.byref(kv), window, sinks, out.data_ptr(), workspace.data_ptr(), workspace.nbytes)
     return out

@@ -41,6 +41,23 @@ class Context:
         h = ctypes.c_void_p()
         check(_lib.lib().wg_init(device, ctypes.byref(h)))
         self.handle = h.value
+        self.lock = threading.Lock()  # a stream choice and the calls that go with it
+
+    def enqueue(self, fn, *args) -> None:
+        """fn(handle, *args) on torch's current stream of this device, as one
+        step for callers on several threads; the caller's current device stays
+        as it was."""
+        import torch
+
+        here = torch.cuda.current_device()
+        s = torch.cuda.current_stream(self.device).cuda_stream if _raw_stream is None else _raw_stream(self.device)
+        with self.lock:
+            _lib.lib().wg_set_stream(self.handle, s if s else _CUDA_STREAM_LEGACY)
+            status = fn(self.handle, *args)
+        if here != self.device:
+            torch.cuda.set_device(here)
+        if status:
+            self._check(status)
 
     def close(self) -> None:
         if self.handle:
@@ -100,6 +117,10 @@ class Context:
 
 
 _CUDA_STREAM_LEGACY = 1  # cudaStreamLegacy
+try:  # the current stream's handle without the stream object around it
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:  # pragma: no cover - no torch, or one without CUDA
+    _raw_stream = None
 
 _contexts: dict[int, Context] = {}
 _ctx_lock = threading.Lock()

@@ -51,35 +51,32 @@ def spec_sample(target: torch.Tensor, draft: torch.Tensor | None, drafts: torch.
     [1][batch][V] (or [batch][V])."""
     if target.dim() == 2 and draft is None:
         target = target.unsqueeze(0)
-    device = target.device
-    if target.dim() != 3 or not target.is_cuda:
+    device = target.get_device()
+    if target.dim() != 3 or device < 0:
         raise _lib.ShapeError(_lib.WG_INVALID_SHAPE, f"target {tuple(target.shape)} must be CUDA logits [k + 1][batch][V]")
-    k, batch, V = target.shape[0] - 1, target.shape[1], target.shape[2]
+    rows, batch, V = target.shape
+    k = rows - 1
     if (draft is None) != (k == 0) or (drafts is None) != (k == 0):
         raise _lib.ShapeError(_lib.WG_INVALID_SHAPE, f"{k} drafted tokens a sequence need their draft logits and drafts")
-    want = [(target, torch.float32, target.shape, "target"), (u, torch.float32, (batch, k + 1), "u")]
+    want = [(target, torch.float32, (rows, batch, V), "target"), (u, torch.float32, (batch, rows), "u")]
     if k:
         want += [(draft, torch.float32, (k, batch, V), "draft"), (drafts, torch.int32, (batch, k), "drafts")]
     if out is None:
-        out = torch.empty((k + 1, batch), dtype=torch.int32, device=device)
+        out = torch.empty((rows, batch), dtype=torch.int32, device=target.device)
     else:
-        want.append((out, torch.int32, (k + 1, batch), "out"))
+        want.append((out, torch.int32, (rows, batch), "out"))
     for t, dt, shape, what in want:
         if t.shape != shape:
-            raise _lib.ShapeError(_lib.WG_INVALID_SHAPE, f"{what} {tuple(t.shape)} must be {tuple(shape)}")
-        if t.dtype != dt or t.device != device or not t.is_contiguous():
-            raise _lib.GpuError(_lib.WG_INVALID_ARGUMENT, f"{what} must be contiguous {dt} on {device}")
-    ctx = context(device.index)
-    ctx.use_torch_stream()
-    L = _lib.lib()
+            raise _lib.ShapeError(_lib.WG_INVALID_SHAPE, f"{what} {tuple(t.shape)} must be {shape}")
+        if t.dtype is not dt or t.get_device() != device or not t.is_contiguous():
+            raise _lib.GpuError(_lib.WG_INVALID_ARGUMENT, f"{what} must be contiguous {dt} on CUDA device {device}")
+    ctx, L = context(device), _lib.lib()
     need = ctypes.c_size_t()
     ctx._check(L.wg_spec_sample_workspace(ctx.handle, batch, k, V, ctypes.byref(need)))
     # from torch's allocator: safe on any stream and inside a graph
-    ws = torch.empty(max(need.value, 8), dtype=torch.uint8, device=device)
-    with torch.cuda.device(device):
-        ctx._check(L.wg_spec_sample(ctx.handle, target.data_ptr(), draft.data_ptr() if k else None,
-                                    drafts.data_ptr() if k else None, batch, k, V, temperature, u.data_ptr(),
-                                    out.data_ptr(), ws.data_ptr(), ws.numel()))
+    ws = torch.empty(max(need.value, 8), dtype=torch.uint8, device=target.device)
+    ctx.enqueue(L.wg_spec_sample, target.data_ptr(), draft.data_ptr() if k else None, drafts.data_ptr() if k else None,
+                batch, k, V, temperature, u.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.nbytes)
     return out
 
 
