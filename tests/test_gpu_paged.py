@@ -96,7 +96,7 @@ CASES = [
     ([1] * 4, [100, 130, 131, 900], 4, 4, 64, 16, 128, 70, BF16),  # sinks past a tile
     ([6] * 3, [0, 250, 777], 8, 2, 64, 48, 100, 3, F16),         # window edges differ by row
     ([4, 1, 9], [500, 2, 64], 12, 4, 128, 32, 33, 1, BF16),
-    ([17], [0], 4, 2, 64, 16, 0, 0, F16),                        # prompts
+    ([17], [0], 4, 2, 64, 16, 0, 0, F16),                        # many rows, little work: the split kernel
     ([64], [0], 32, 8, 128, 64, 0, 0, F16),
     ([130], [0], 8, 2, 128, 16, 0, 0, BF16),
     ([257], [100], 6, 3, 64, 48, 0, 0, F16),
@@ -107,6 +107,22 @@ CASES = [
     ([260], [700], 14, 2, 64, 16, 129, 5, BF16),
     ([333, 40], [1, 900], 8, 1, 128, 32, 200, 130, F16),
     ([140], [60], 2, 1, 256, 16, 64, 4, BF16),
+    # prompts: work enough for the tensor-core kernel
+    ([130], [0], 32, 8, 128, 64, 0, 0, F16),
+    ([300], [0], 32, 8, 64, 16, 0, 0, BF16),
+    ([200], [1000], 32, 32, 128, 128, 0, 0, F16),                # one head a KV head: 256 rows a unit
+    ([65] * 4, [0, 1, 63, 500], 16, 4, 128, 48, 0, 0, BF16),
+    ([100, 1, 0, 300], [0, 50, 7, 129], 56, 8, 64, 32, 0, 0, F16),  # 7 heads: 126 of a tile's 128 rows
+    ([257], [100], 24, 8, 64, 80, 0, 0, F16),
+    ([80], [300], 32, 8, 256, 64, 0, 0, F16),
+    ([33, 64], [0, 99], 40, 2, 256, 16, 0, 0, BF16),             # 20 heads a KV head
+    ([40], [600], 128, 1, 128, 16, 0, 0, F16),                   # 128 heads: a row a tile
+    ([300], [0], 32, 8, 128, 64, 50, 0, F16),                    # windows: their edges, sinks, freed pages
+    ([260], [700], 28, 4, 64, 16, 129, 5, BF16),
+    ([333, 40], [1, 900], 24, 3, 128, 32, 200, 130, F16),
+    ([140], [60], 32, 8, 256, 16, 64, 4, BF16),
+    ([200] * 2, [5, 2000], 32, 8, 64, 64, 1, 1, F16),
+    ([3] * 90, list(range(0, 1800, 20)), 32, 8, 128, 16, 0, 0, F16),  # many short ones
 ]
 
 
@@ -128,7 +144,8 @@ def test_what_later_rows_see_does_not_touch_earlier_ones(rows, Dh, page, dtype, 
     """A key / value of position p holds inf or NaN: rows before p are exact,
     and so are rows whose window has left it behind."""
     window, pos, hot = 24, 37, 37 + rows // 2
-    q, k, v, table = make([rows], [pos], 4, 2, Dh, page, dtype, seed=rows, window=window, sinks=2)
+    # (64 heads: the longer ones go to the tensor-core kernel)
+    q, k, v, table = make([rows], [pos], 64, 32, Dh, page, dtype, seed=rows, window=window, sinks=2)
     clean_k, clean_v = k.clone(), v.clone()
     pg = table[0, hot // page]
     k[pg, :, hot % page] = bad
@@ -161,7 +178,7 @@ def test_rows_that_see_nothing_and_rows_of_nobody():
 
 
 def test_a_long_prompt_with_padding_rows_first():
-    H, Hkv, Dh, page = 4, 2, 128, 32
+    H, Hkv, Dh, page = 32, 16, 128, 32
     q, k, v, table = make([200], [0], H, Hkv, Dh, page, F16)
     out = paged.attention_paged(q, torch.tensor([-130], dtype=torch.int32, device="cuda"), k, v, table)
     assert not out[:130].any()
@@ -179,7 +196,7 @@ def test_missing_pages_are_left_out_and_reported():
             wg.context().sync()
         check(out, q, k, v, table, counts, pos)
     # a long prompt
-    q, k, v, table = make([300], [50], H, Hkv, Dh, page, F16)
+    q, k, v, table = make([300], [50], 64, 16, Dh, page, F16)
     table[0, 5] = -1
     out = run(q, k, v, table, [300], [50])
     with pytest.raises(wg.GpuError):
@@ -224,7 +241,7 @@ def test_offsets_past_32_bits():
     for rows in (1, 150):
         n = 500
         table = torch.arange(pages - 10, pages, dtype=torch.int32, device="cuda").view(1, -1)
-        q = (torch.randn((rows, 16, Dh), generator=gen(3), device="cuda") / 8).to(F16)
+        q = (torch.randn((rows, 32, Dh), generator=gen(3), device="cuda") / 8).to(F16)
         out = run(q, k, v, table, [rows], [n - rows])
         check(out, q, k[-40:], v[-40:], table - (pages - 40), [rows], [n - rows])
     qkv = torch.randn((1, (16 + 2 * Hkv) * Dh), device="cuda")
@@ -257,7 +274,7 @@ def test_many_sequences():
 def test_streams_and_graphs(rows):
     """On a side stream, captured, and two graphs replayed at once: each call
     has its own workspace."""
-    counts, H, Hkv, Dh, page = [rows] * 2, 8, 1, 128, 64
+    counts, H, Hkv, Dh, page = [rows] * 2, 16, 2, 128, 64
     a = make(counts, [1500, 700], H, Hkv, Dh, page, F16, seed=1)
     b = make(counts, [900, 2222], H, Hkv, Dh, page, F16, seed=2)
     pa = torch.tensor([1500, 700], dtype=torch.int32, device="cuda")

@@ -265,6 +265,11 @@ struct SplitCfg {
   static constexpr int kWarps = 4 * MT;            // consumers
   static constexpr int kThreads = (kWarps + 1) * 32;
   static constexpr int kCtas = MT == 1 && Dh <= 128 ? 2 : 1;  // per SM
+  // With eight consumer warps the queries' fragments are read from shared memory
+  // with each tile: in registers too they spill (verify rows: 39 us, so 36).
+  static constexpr bool kQSmem = MT == 2;
+  static constexpr int kQRow = Dh + 8;
+  static constexpr int kQBytes = kQSmem ? kRows * kQRow * 2 : 0;
   static constexpr int kTileBytes = kKeys * Dh * 2;  // K or V of a stage
   static constexpr int kStageBytes = 2 * kTileBytes;
   // The warps' merge: two sets of the rows' sums, 8 floats between rows (the 8
@@ -272,7 +277,7 @@ struct SplitCfg {
   // same memory stages the queries, and P where a V row is odd.
   static constexpr int kRedRow = Dh + 8;
   static constexpr int kRedBytes = 2 * kRows * kRedRow * 4;
-  static constexpr int kFixed = 1024 /* alignment */ + kRedBytes + 4 * 4 * kRows * 2 + 256;
+  static constexpr int kFixed = 1024 /* alignment */ + kRedBytes + kQBytes + 4 * 4 * kRows * 2 + 256;
   static constexpr int kBudget = 224 * 1024 / kCtas - 1024;
   static constexpr int kFit = (kBudget - kFixed) / kStageBytes;
   static constexpr int kStages = kFit > kMaxStages ? kMaxStages : kFit;
@@ -295,6 +300,7 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
   float *red = reinterpret_cast<float *>(smem + (size_t)S * C::kStageBytes);  // [2][kRows][kRedRow]
   float *sm_m = red + 2 * C::kRows * C::kRedRow;           // [4 key groups][kRows]
   float *sm_l = sm_m + 4 * C::kRows;
+  T *sq = reinterpret_cast<T *>(C::kQSmem ? sm_l + 4 * C::kRows : red);  // [kRows][kQRow]
   __shared__ uint64_t full[S], empty[S];
   __shared__ int held[S];                          // which 16-key groups of a stage's pages were loaded
   __shared__ int scan_red[C::kThreads / 32];
@@ -466,8 +472,6 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
       // queries, 16 bytes a load, through the merge buffer into A fragments; the
       // position of each of this thread's rows
       auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(C::kWarps * 32) : "memory"); };
-      T *sq = reinterpret_cast<T *>(red);
-      constexpr int kQRow = Dh + 8;
       for (int i = tid; i < C::kRows * (Dh / 8); i += C::kWarps * 32) {
         const int row = i / (Dh / 8), ch = i - row * (Dh / 8), m = m0 + row, qi = m / A.G;
         uint4 v = make_uint4(0, 0, 0, 0);
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
           v = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(A.q) +
                                                     ((size_t)(w.r0 + qi) * A.H + hk * A.G + (m - qi * A.G)) * Dh) +
                     ch);
-        *reinterpret_cast<uint4 *>(sq + row * kQRow + ch * 8) = v;
+        *reinterpret_cast<uint4 *>(sq + row * C::kQRow + ch * 8) = v;
       }
       int rp[2];
 #pragma unroll
@@ -484,16 +488,21 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
         rp[e] = (int)max(-1LL, min(i < w.n ? (long long)w.p + i : -1LL, 0x7ffffffeLL));
       }
       sync();
-      uint32_t qa[Dh / 16][4];
+      const uint32_t q_at = smem_u32(sq + (wr * 16 + (jm & 1) * 8 + jr) * C::kQRow + (jm >> 1) * 8);
+      uint32_t qa[C::kQSmem ? 1 : Dh / 16][4];
+      if constexpr (!C::kQSmem) {
 #pragma unroll
-      for (int kk = 0; kk < Dh / 16; kk++)
-        ldsm4(smem_u32(sq + (wr * 16 + (jm & 1) * 8 + jr) * kQRow + kk * 16 + (jm >> 1) * 8), qa[kk]);
-      sync();  // the buffer is free again
+        for (int kk = 0; kk < Dh / 16; kk++) ldsm4(q_at + kk * 32, qa[kk]);
+        sync();  // the buffer is free again
+      }
       float o[Dh / 8][4];
       float mx[2] = {-INFINITY, -INFINITY}, ls[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int d = 0; d < Dh / 8; d++) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
-      const long long p_last = (long long)w.p + w.n - 1;
+      // keys that every row sees: up to open_to, and from open_from on or sinks
+      const int open_to = max(-1, w.p - (KW - 1));
+      const int open_from = A.window > 0 ? (int)max(0LL, (long long)w.p + w.n - A.window) : 0;
+      const int open_sinks = A.sinks - (KW - 1);
 
       for (int t = t0; t < t1; t++) {
         wait(&full[stage], phase);
@@ -504,9 +513,7 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
           uint8_t *stage_v = smem + (size_t)stage * C::kStageBytes + C::kTileBytes;
           const uint32_t kaddr = smem_u32(smem) + (uint32_t)stage * C::kStageBytes;
           const uint32_t vaddr = kaddr + C::kTileBytes;
-          // every row sees every one of the keys
-          const bool open = key0 + KW - 1 <= w.p && have == kAll &&
-                            (A.window == 0 || key0 + KW - 1 < A.sinks || (long long)key0 > p_last - A.window);
+          const bool open = key0 <= open_to && have == kAll && (key0 >= open_from || key0 < open_sinks);
           // whether some row of the sequence sees key i of these
           auto seen = [&](int i) {
             const int key = key0 + i;
@@ -537,13 +544,15 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
 #pragma unroll
           for (int kk = 0; kk < Dh / 16; kk++) {
             const int ch = 2 * kk + (jm & 1);
+            if constexpr (C::kQSmem) ldsm4(q_at + kk * 32, qa[0]);
+            const uint32_t(&qk)[4] = qa[C::kQSmem ? 0 : kk];
 #pragma unroll
             for (int np = 0; np < KW / 16; np++) {
               const int row = wk * KW + np * 16 + 8 * (jm >> 1) + jr;
               uint32_t bf[4];
               ldsm4(kaddr + (ch >> 3) * kBlkBytes + row * 128 + (((ch & 7) ^ (row & 7)) << 4), bf);
-              mma16816<T>(s[2 * np], qa[kk], bf[0], bf[1]);
-              mma16816<T>(s[2 * np + 1], qa[kk], bf[2], bf[3]);
+              mma16816<T>(s[2 * np], qk, bf[0], bf[1]);
+              mma16816<T>(s[2 * np + 1], qk, bf[2], bf[3]);
             }
           }
           if (!open) {
@@ -911,8 +920,7 @@ cudaError_t launch_paged_rope_kv(const float *qkv, const PagedRows &rows, int H,
 }
 
 size_t paged_attention_workspace(int Dh, int num_sms) {
-  // the larger of the 16-row (two CTAs an SM, but for Dh = 256) and the 32-row
-  // kernels' needs: the same number of rows in all
+  // two CTAs an SM of 16 rows, or one of 32
   const size_t P = (size_t)num_sms * 2;
   return P * 8 * sizeof(int) + 2 * P * 16 * (size_t)(Dh + 2) * sizeof(float);
 }
@@ -920,7 +928,7 @@ size_t paged_attention_workspace(int Dh, int num_sms) {
 cudaError_t launch_paged_attention(const void *q, const PagedRows &rows, int H, int Hkv, int Dh,
                                    const wg_paged_kv &kv, int window, int sinks, void *out, void *workspace,
                                    unsigned *flags, int num_sms, cudaStream_t s, bool pdl) {
-  if (paged_prompt_supported(rows, H, Hkv, num_sms))
+  if (paged_prompt_wins(rows, H, Hkv, Dh, num_sms))
     return launch_paged_prompt(q, rows, H, Hkv, Dh, kv, window, sinks, out, flags, num_sms, s, pdl);
   SplitArgs A{};
   A.pr = rows;

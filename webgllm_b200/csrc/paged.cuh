@@ -32,8 +32,8 @@ cudaError_t launch_paged_attention(const void *q, const PagedRows &rows, int H, 
                                    unsigned *flags, int num_sms, cudaStream_t s, bool pdl);
 
 // Many rows a sequence (paged_prompt_sm100.cu): launch_paged_attention sends the
-// shapes that this accepts there.
-bool paged_prompt_supported(const PagedRows &rows, int H, int Hkv, int num_sms);
+// shapes there for which this says so.
+bool paged_prompt_wins(const PagedRows &rows, int H, int Hkv, int Dh, int num_sms);
 cudaError_t launch_paged_prompt(const void *q, const PagedRows &rows, int H, int Hkv, int Dh, const wg_paged_kv &kv,
                                 int window, int sinks, void *out, unsigned *flags, int num_sms, cudaStream_t s,
                                 bool pdl);

@@ -628,13 +628,13 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
           if (j > 0 || part > 0) {
             sum = exps();
             holds = sum <= 256.0f;
-            if (ref == -INFINITY) {  // nothing seen so far: still so? (rows of nobody: always)
+            if (p < 0) {
+              holds = true;  // (rows of nobody hold anything: they decide nothing for their warp)
+            } else if (ref == -INFINITY) {  // nothing seen so far: still so?
               float top = -INFINITY;
-              if (p >= 0) {
 #pragma unroll
-                for (int c = 0; c < 64; c += 2) top = max3(top, sp[c], sp[c + 1]);
-              }
-              holds = !(top > -INFINITY) && (p < 0 || !isnan(sum));
+              for (int c = 0; c < 64; c += 2) top = max3(top, sp[c], sp[c + 1]);
+              holds = !(top > -INFINITY) && !isnan(sum);
             }
           }
           if (!__all_sync(0xffffffffu, holds)) {
@@ -769,10 +769,22 @@ cudaError_t prompt_t(const void *q, PromptArgs A, const wg_paged_kv &kv, int num
 
 }  // namespace
 
-bool paged_prompt_supported(const PagedRows &rows, int H, int Hkv, int num_sms) {
-  (void)num_sms;
+// Which of the two kernels, from the rows a sequence has on average (lengths are
+// on the device, and both kernels' times are proportional to them). This one
+// takes rounds of num_sms units of 256 rows (128 at Dh = 256), a CTA for all keys
+// of a unit; the split kernel spreads row tiles of 32 (16 at Dh = 256) over the
+// machine. Per 64 keys, a round here costs what kSplitWorth row tiles an SM cost
+// there (8 sequences x 4096 keys, Dh = 128, 8 KV heads of 4: 16 rows 65 us here and
+// 88 us there, 8 rows 65 and 54; one sequence of 128 rows 63 and 88 us, of 64 rows
+// 62 and 53; Dh = 64, 8 sequences: 32 rows 68 and 89 us, 16 rows 67 and 59).
+bool paged_prompt_wins(const PagedRows &rows, int H, int Hkv, int Dh, int num_sms) {
   const int G = H / Hkv;
-  return G <= 128 && (long long)rows.rows / rows.batch * G >= 64;
+  if (G > 128) return false;  // a tile of 128 rows holds no whole row of such a group
+  const double kSplitWorth = Dh == 64 ? 1.46 : Dh == 128 ? 0.79 : 0.82;
+  const long long n = (rows.rows + rows.batch - 1) / rows.batch, heads = (long long)rows.batch * Hkv;
+  const long long unit = (Dh == 256 ? 1 : 2) * (128 / G), tile = Dh == 256 ? 16 : 32;
+  const long long units = heads * ((n + unit - 1) / unit), tiles = heads * ((n * G + tile - 1) / tile);
+  return (double)((units + num_sms - 1) / num_sms) * num_sms * kSplitWorth < (double)tiles;
 }
 
 cudaError_t launch_paged_prompt(const void *q, const PagedRows &rows, int H, int Hkv, int Dh, const wg_paged_kv &kv,
