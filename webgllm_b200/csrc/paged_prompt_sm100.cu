@@ -780,8 +780,9 @@ cudaError_t prompt_t(const void *q, PromptArgs A, const wg_paged_kv &kv, int num
 bool paged_prompt_wins(const PagedRows &rows, int H, int Hkv, int Dh, int num_sms) {
   const int G = H / Hkv;
   if (G > 128) return false;  // a tile of 128 rows holds no whole row of such a group
-  const double kSplitWorth = Dh == 64 ? 1.46 : Dh == 128 ? 0.79 : 0.82;
   const long long n = (rows.rows + rows.batch - 1) / rows.batch, heads = (long long)rows.batch * Hkv;
+  if (n * G <= 16) return false;  // one 16-row tile: K and V are read once, at the memory's rate
+  const double kSplitWorth = Dh == 64 ? 1.46 : Dh == 128 ? 0.79 : 0.82;
   const long long unit = (Dh == 256 ? 1 : 2) * (128 / G), tile = Dh == 256 ? 16 : 32;
   const long long units = heads * ((n + unit - 1) / unit), tiles = heads * ((n * G + tile - 1) / tile);
   return (double)((units + num_sms - 1) / num_sms) * num_sms * kSplitWorth < (double)tiles;
