@@ -47,15 +47,13 @@ class Context:
         """fn(handle, *args) on torch's current stream of this device, as one
         step for callers on several threads; the caller's current device stays
         as it was."""
-        import torch
-
-        here = torch.cuda.current_device()
-        s = torch.cuda.current_stream(self.device).cuda_stream if _raw_stream is None else _raw_stream(self.device)
+        here = _current_device()
+        stream = _raw_stream(self.device)
         with self.lock:
-            _lib.lib().wg_set_stream(self.handle, s if s else _CUDA_STREAM_LEGACY)
+            _lib.lib().wg_set_stream(self.handle, stream if stream else _CUDA_STREAM_LEGACY)
             status = fn(self.handle, *args)
         if here != self.device:
-            torch.cuda.set_device(here)
+            _set_device(here)
         if status:
             self._check(status)
 
@@ -117,10 +115,32 @@ class Context:
 
 
 _CUDA_STREAM_LEGACY = 1  # cudaStreamLegacy
-try:  # the current stream's handle without the stream object around it
-    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+
+
+def _raw_stream(device: int) -> int:
+    """The handle of torch's current stream of a device (0: the default one)."""
+    import torch
+
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _current_device() -> int:
+    import torch
+
+    return torch.cuda.current_device()
+
+
+def _set_device(device: int) -> None:
+    import torch
+
+    torch.cuda.set_device(device)
+
+
+try:  # the same without the Python objects around them
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream  # noqa: F811
+    from torch._C import _cuda_getDevice as _current_device  # noqa: F811
 except ImportError:  # pragma: no cover - no torch, or one without CUDA
-    _raw_stream = None
+    pass
 
 _contexts: dict[int, Context] = {}
 _ctx_lock = threading.Lock()
@@ -128,6 +148,9 @@ _ctx_lock = threading.Lock()
 
 def context(device: int | None = None) -> Context:
     """The per-device default context."""
+    ctx = _contexts.get(device)  # (None: no device given, or none made yet)
+    if ctx is not None:
+        return ctx
     if device is None:
         import torch
 
