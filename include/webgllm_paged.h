@@ -66,7 +66,8 @@ int wg_paged_rope_kv(wg_ctx *ctx, const float *qkv, int rows, int batch, const i
  * the cache's dtype. Dh in {64, 128, 256}, H a multiple of Hkv, any rows per sequence
  * (one for a decode step, k + 1 to verify drafts, a prompt's chunk). What a
  * row does not see may hold anything, NaN included. A visible position whose
- * page entry names no page is left out and reported by wg_sync.
+ * page entry names no page is left out and reported by wg_sync; positions
+ * past the table are left out.
  * `workspace` (16-byte aligned device memory of at least
  * wg_paged_attention_workspace bytes, any content) holds the partial sums of
  * sequences that several CTAs share: calls that may overlap on the GPU need

@@ -185,6 +185,27 @@ def test_a_long_prompt_with_padding_rows_first():
     check(out[130:], q[130:], k, v, table, [70], [0])
 
 
+@pytest.mark.parametrize("rows", [1, 3, 160])
+def test_extreme_positions(rows):
+    """The first and last positions an int32 holds: padding, and rows past the
+    end of their table, which see all of it (or nothing through a window)."""
+    H, Hkv, Dh, page, n = 32, 16, 128, 16, 64
+    low, high = -2 ** 31, 2 ** 31 - 1
+    # (every row of a sequence at `high` sees the whole table: 64 positions of data)
+    q, k, v, table = make([1] * (3 * rows), [n - 1] * (3 * rows), H, Hkv, Dh, page, F16)
+    table = table[[0, rows, 2 * rows]].contiguous()
+    pos = torch.tensor([low, high, high - rows + 1], dtype=torch.int32, device="cuda")
+    out = paged.attention_paged(q, pos, k, v, table)
+    assert not out[:rows].any()
+    check(out[rows:], q[rows:], k, v, table[[1] * rows + [2] * rows].contiguous(), [1] * (2 * rows), [n - 1] * (2 * rows))
+    for window in (5, high):
+        out = paged.attention_paged(q, pos, k, v, table, window=window)
+        assert not out[:rows].any()
+        if window == 5:
+            assert not out.any()
+    wg.context().sync()
+
+
 def test_missing_pages_are_left_out_and_reported():
     counts, pos, H, Hkv, Dh, page = [1, 2], [100, 75], 8, 2, 64, 16
     for bad in (-1, 10 ** 6):

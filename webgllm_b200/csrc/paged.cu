@@ -194,9 +194,9 @@ __global__ void __launch_bounds__(256)
 //                   (wait, scores, maximum, exponentials, P V) takes a warp
 //                   about 2000 cycles whatever KW is, so small heads take 32
 //                   keys at a time (Dh = 64, 32 sequences with a window of 4096:
-//                   WIN16 us with 16 keys, WIN32 us with 32), and 32 query rows
+//                   59 us with 16 keys, 53 with 32), and 32 query rows
 //                   take eight warps (five rows of 4 heads, 8 sequences of 4k:
-//                   VER4 us with four warps of both row tiles, VER8 us).
+//                   52 us with four warps of both row tiles, 39 with eight).
 // P stays at fp32 precision: hi + lo 16-bit halves, two products (the tensor
 // pipe idles under the loads).
 // A (sequence, head, rows) unit that one CTA finishes alone is written by it;
@@ -500,8 +500,8 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
 #pragma unroll
       for (int d = 0; d < Dh / 8; d++) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
       // keys that every row sees: up to open_to, and from open_from on or sinks
-      const int open_to = max(-1, w.p - (KW - 1));
-      const int open_from = A.window > 0 ? (int)max(0LL, (long long)w.p + w.n - A.window) : 0;
+      const int open_to = (int)max(-1LL, (long long)w.p - (KW - 1));
+      const int open_from = A.window > 0 ? (int)min(max(0LL, (long long)w.p + w.n - A.window), 0x7fffffffLL) : 0;
       const int open_sinks = A.sinks - (KW - 1);
 
       for (int t = t0; t < t1; t++) {

@@ -11,10 +11,10 @@
 //                scores, mask, maximum, exp2, P as 16-bit pairs back into the
 //                scores' tensor-memory columns (the A operand of P V), the row
 //                sum in a register; at the end O from tensor memory to `out`.
-//                The reference maximum follows the true one only when that
-//                has grown by 2^8 (P stays below 2^8, well inside fp16): O is
-//                then rescaled in tensor memory, which almost never happens
-//                after the first tiles;
+//                The reference of the exponentials is the first tiles' maximum
+//                and follows only when a tile's P adds up to more than 2^8
+//                (so P stays well inside fp16): O is then rescaled in tensor
+//                memory, which almost never happens after the first tiles;
 //   one warp     MMA: one thread issues S_t = Q_t K^T (both operands in shared
 //                memory) and O_t += P_t V (P from tensor memory, V as it lies,
 //                [key][dim], the MN-major form). The two tiles alternate:
