@@ -50,3 +50,51 @@ def test_cache_shapes_are_checked_before_the_device():
         paged.attention_paged(q.float(), pos, k.float(), v.float(), table)
     with pytest.raises(wg.GpuError):
         paged.attention_paged(q, pos, k, v.bfloat16(), table)
+
+
+def cache(pages=6, batch=2, max_len=100, page=16):
+    return paged.PagedCache(1, batch, 2, 64, pages, max_len, page_size=page, device="cpu")
+
+
+def test_pages_are_handed_out_and_taken_back():
+    c = cache()
+    assert c.max_pages == 7 and c.max_len == 112
+    c.reserve(0, 33)  # 3 pages
+    c.reserve(0, 40)  # which hold 40 already
+    c.reserve(1, 1)
+    assert (c.table[0, :3] >= 0).all() and (c.table[0, 3:] < 0).all() and len(c.free) == 2
+    held = c.table[c.table >= 0].tolist()
+    assert len(set(held)) == 4
+    with pytest.raises(wg.GpuError) as e:
+        c.reserve(1, 65)  # 4 more: only 2 free
+    assert e.value.code == _lib.WG_OUT_OF_MEMORY and len(c.free) == 2 and (c.table[1, 1:] < 0).all()
+    c.release(0)
+    assert len(c.free) == 5 and (c.table[0] < 0).all()
+    c.reserve(1, 65)
+    assert (c.table[1, :5] >= 0).all() and len(c.free) == 1
+    c.release(1)
+    c.release(1)
+    assert sorted(c.free) == list(range(6))
+
+
+def test_trim_keeps_the_window_and_the_sinks():
+    c = cache(pages=7, batch=1)
+    c.reserve(0, 112)
+    # a row at 80 with a window of 20 sees 61..80 and the sinks 0..16
+    assert c.trim(0, 80, 20, 17) == 1  # page 2 (32..47); page 3 (48..63) is still seen
+    assert c.host[0][2] < 0 and all(c.host[0][i] >= 0 for i in (0, 1, 3, 4, 5, 6))
+    assert c.trim(0, 80, 20, 17) == 0
+    assert c.trim(0, 111, 16, 0) == 5  # pages 0, 1, 3, 4, 5; the window begins at page 6
+    assert c.trim(0, 111, 0) == 0  # no window: everything is seen
+    c.reserve(0, 112, start=96)
+    assert len(c.free) == 6
+
+
+def test_cache_refusals():
+    for kw in (dict(page=24), dict(page=0), dict(pages=0), dict(batch=0), dict(max_len=0)):
+        with pytest.raises(wg.ShapeError):
+            cache(**kw)
+    with pytest.raises(wg.GpuError):
+        paged.PagedCache(1, 1, 1, 64, 4, 64, dtype=torch.float32, device="cpu")
+    with pytest.raises(wg.RangeError):
+        cache().reserve(0, 113)

@@ -11,8 +11,10 @@ quantised to Q4_0 by the llama.cpp rule on the device.
 A decode step is captured once as a CUDA graph and replayed: the token ids
 (argmax) and the positions live on the device, so no host round trip is
 needed between tokens. `batch` independent sequences decode together (one
-row each), and with `tp` (a webgllm_b200.comm.TensorGroup) the model is split
-across the GPUs of a node (webgllm_b200.tp): per layer two row-parallel sums
+row each), with `cache` (a webgllm_b200.paged.PagedCache) their keys and
+values live in pages instead of one run of max_ctx positions each, seen in
+full or through a sliding window with sinks, and with `tp` (a
+webgllm_b200.comm.TensorGroup) the model is split across the GPUs of a node (webgllm_b200.tp): per layer two row-parallel sums
 (the push exchange for decode rows, NCCL's all-reduce through the library
 for prompt rows) and one MAX all-reduce for the greedy pick.
 """
@@ -28,6 +30,7 @@ from . import _lib
 from . import tp as TP
 from .q4 import QuantMatrix, context, newQuantMatrix, packQ4_0
 from ._lib import WG_F16, WG_F32, WG_PRO_RMSNORM, WG_PRO_SWIGLU
+from .paged import workspace_bytes
 
 P = ctypes.c_void_p
 
@@ -132,11 +135,16 @@ class DecoderModel:
 
     tp: None, or this rank's webgllm_b200.comm.TensorGroup; every rank
     draws the same full random weights and keeps its shard (webgllm_b200.tp),
-    so the model is the same for every world size."""
+    so the model is the same for every world size.
+    cache: None (contiguous caches of max_ctx positions), or a PagedCache with
+    this model's attention layers, local KV heads and batch; the caller reserves
+    its pages ahead of the positions a forward reaches. window / sinks: with a
+    cache, rows see the last `window` positions and the first `sinks` ones
+    (window 0: all)."""
 
     def __init__(self, cfg: DecoderConfig, seed: int = 0, max_ctx: int = 1024, max_rows: int = 512,
                  keep_blocks: bool = False, device: int | None = None, fused: bool = True, batch: int = 1,
-                 tp=None, push: bool = True):
+                 tp=None, push: bool = True, cache=None, window: int = 0, sinks: int = 0):
         self.cfg = cfg
         self.fused = fused
         self.batch = batch
@@ -193,8 +201,21 @@ class DecoderModel:
             L["down"] = lin(D, I, cols=TP.down_cols(cfg, sh) if sh else None)
             self.layers.append(L)
         B = batch
-        self.k_cache = torch.zeros((max(n_attn, 1), B, self.Hkv, max_ctx, Dh), dtype=torch.float16, device="cuda")
-        self.v_cache = torch.zeros_like(self.k_cache)
+        self.cache, self.window, self.sinks = cache, window, sinks
+        if cache is None:
+            if window or sinks:
+                raise ValueError("a sliding window needs a paged cache")
+            self.k_cache = torch.zeros((max(n_attn, 1), B, self.Hkv, max_ctx, Dh), dtype=torch.float16, device="cuda")
+            self.v_cache = torch.zeros_like(self.k_cache)
+        else:
+            shape = (max(n_attn, 1), self.Hkv, Dh)
+            if (cache.k.shape[0], cache.k.shape[2], cache.k.shape[4]) != shape or cache.batch != B \
+                    or cache.k.dtype != torch.float16 or cache.k.get_device() != self.ctx.device:
+                raise ValueError(f"the cache must hold {shape[0]} layers, {B} sequences and {self.Hkv} heads of {Dh} in "
+                                 f"float16 on device {self.ctx.device}")
+            self.max_ctx = cache.max_len
+            self.pages = [cache.layer(i) for i in range(n_attn)]
+            self.attn_ws = torch.empty(workspace_bytes(self.ctx.device, Dh), dtype=torch.uint8, device="cuda")
         self.conv_state = torch.zeros((max(n_conv, 1), B, cfg.conv_width - 1, D), dtype=torch.float16,
                                       device="cuda")
         # activations for up to max_rows rows
@@ -223,6 +244,7 @@ class DecoderModel:
         # speculative verification: greedy picks after every row of each
         # sequence, [rows per sequence][batch] (None: the last row only)
         self.row_picks = None
+        self.row_logits = None  # where a forward leaves its logits instead of `logits`: [rows per sequence][batch][V]
         self.row_keys = None  # their packed keys under tensor parallelism, [rows per sequence][batch]
         # speculative decoding of conv models: the conv state after each draft
         # token ([conv layers][batch][slots][W-1][D]) and where this forward's
@@ -253,8 +275,9 @@ class DecoderModel:
 
     def reset(self):
         self.pos.zero_()
-        self.k_cache.zero_()
-        self.v_cache.zero_()
+        if self.cache is None:  # (pages are never read past what was appended)
+            self.k_cache.zero_()
+            self.v_cache.zero_()
         self.conv_state.zero_()
 
     def _mm_norm(self, lin: Linear, resid, add, w, resid_out, y: torch.Tensor, rows: int):
@@ -303,8 +326,17 @@ class DecoderModel:
         cfg, L, c = self.cfg, _lib.lib(), P(self.ctx.handle)
         H, Hkv, Dh = self.H, self.Hkv, cfg.head_dim
         s = lay["slot"]
-        kc, vc = self.k_cache[s], self.v_cache[s]
         qn, kn = lay.get("q_norm"), lay.get("k_norm")
+        if self.cache is not None:
+            kv = ctypes.byref(self.pages[s])
+            self._c(L.wg_paged_rope_kv(c, self.qkv.data_ptr(), rows, self.batch, None, H, Hkv, Dh, self.pos.data_ptr(),
+                                       cfg.theta, qn.data_ptr() if qn is not None else None,
+                                       kn.data_ptr() if kn is not None else None, cfg.eps, self.q.data_ptr(), kv))
+            self._c(L.wg_paged_attention(c, self.q.data_ptr(), rows, self.batch, None, H, Hkv, Dh, self.pos.data_ptr(),
+                                         kv, self.window, self.sinks, self.att.data_ptr(), self.attn_ws.data_ptr(),
+                                         self.attn_ws.numel()))
+            return
+        kc, vc = self.k_cache[s], self.v_cache[s]
         # decode of up to 8 sequences: one launch (measured: configs 2 / 3
         # gain 3-5 %; config 4 at batch 8, with the tensor-core attention,
         # 3.07 -> 3.00 ms a step)
@@ -409,9 +441,10 @@ class DecoderModel:
         sharded = self.world > 1
 
         def head(j, argmax, keys):
+            logits = self.logits if self.row_logits is None else self.row_logits[j]
             self._c(L.wg_head_rmsnorm(c, P(cur[j].data_ptr()), P(add[j].data_ptr() if add is not None else None),
                                       P(self.final_norm.data_ptr()), cfg.eps, B, rps, cfg.hidden,
-                                      P(self.head.data_ptr()), self.V, self.vocab_offset, P(self.logits.data_ptr()),
+                                      P(self.head.data_ptr()), self.V, self.vocab_offset, P(logits.data_ptr()),
                                       P(argmax), P(keys)))
 
         if self.row_picks is not None:

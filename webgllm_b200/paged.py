@@ -22,7 +22,7 @@ from . import _lib
 from ._lib import WG_BF16, WG_F16, GpuError, ShapeError, wg_paged_kv
 from .q4 import context
 
-__all__ = ["attention_paged", "rope_kv_paged"]
+__all__ = ["PagedCache", "attention_paged", "rope_kv_paged"]
 
 _CODES = {torch.float16: WG_F16, torch.bfloat16: WG_BF16}
 _workspace_bytes: dict = {}  # (device, head dim) -> bytes
@@ -149,3 +149,72 @@ def attention_paged(q: torch.Tensor, pos: torch.Tensor, k: torch.Tensor, v: torc
     context(device).enqueue(_lib.lib().wg_paged_attention, q.data_ptr(), rows, batch, rs, heads, hkv, dim, p,
                             ctypes.byref(kv), window, sinks, out.data_ptr(), workspace.data_ptr(), workspace.nbytes)
     return out
+
+
+class PagedCache:
+    """The pages of `layers` attention layers and the table that says which
+    sequence holds which (one table for all layers: a page is the same slots in
+    each). Bookkeeping is on the host; the table's device copy is updated on
+    torch's current stream, so work enqueued before still sees the old one."""
+
+    def __init__(self, layers: int, batch: int, kv_heads: int, head_dim: int, num_pages: int, max_len: int,
+                 page_size: int = 64, dtype: torch.dtype = torch.float16, device="cuda"):
+        if page_size <= 0 or page_size % 16:
+            raise _bad(f"page size {page_size} must be a multiple of 16")
+        if dtype not in _CODES:
+            raise _arg(f"pages must be float16 or bfloat16, not {dtype}")
+        if min(layers, batch, kv_heads, num_pages, max_len) <= 0:
+            raise _bad(f"{layers} layers, {batch} sequences, {kv_heads} heads, {num_pages} pages, length {max_len}")
+        self.page_size, self.batch, self.num_pages = page_size, batch, num_pages
+        self.max_pages = -(-max_len // page_size)
+        self.max_len = self.max_pages * page_size
+        self.k = torch.empty((layers, num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+        self.v = torch.empty_like(self.k)
+        self.table = torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=device)
+        self.host = [[-1] * self.max_pages for _ in range(batch)]
+        self.free = list(range(num_pages - 1, -1, -1))
+
+    def _upload(self, rows) -> None:
+        for b in rows:
+            self.table[b].copy_(torch.tensor(self.host[b], dtype=torch.int32))
+
+    def reserve(self, b: int, length: int, start: int = 0) -> None:
+        """Pages for positions start .. length - 1 of sequence b (those it has
+        it keeps). Without enough free pages nothing changes and
+        GpuError(WG_OUT_OF_MEMORY) is raised."""
+        if not 0 <= start <= length <= self.max_len:
+            raise _lib.RangeError(_lib.WG_OUT_OF_RANGE, f"positions {start}..{length} of {self.max_len}")
+        need = [i for i in range(start // self.page_size, -(-length // self.page_size)) if self.host[b][i] < 0]
+        if len(need) > len(self.free):
+            raise GpuError(_lib.WG_OUT_OF_MEMORY, f"{len(need)} pages needed, {len(self.free)} of {self.num_pages} free")
+        for i in need:
+            self.host[b][i] = self.free.pop()
+        if need:
+            self._upload([b])
+
+    def trim(self, b: int, position: int, window: int, sinks: int = 0) -> int:
+        """Takes back the pages of sequence b that no row at `position` or later
+        sees through the window and the sinks; returns how many."""
+        if window <= 0:
+            return 0
+        gone = 0
+        for i in range(-(-sinks // self.page_size), max(0, position - window + 1) // self.page_size):
+            if self.host[b][i] >= 0:
+                self.free.append(self.host[b][i])
+                self.host[b][i] = -1
+                gone += 1
+        if gone:
+            self._upload([b])
+        return gone
+
+    def release(self, b: int) -> None:
+        """Takes back all pages of sequence b."""
+        held = [i for i in self.host[b] if i >= 0]
+        if held:
+            self.free += held
+            self.host[b] = [-1] * self.max_pages
+            self._upload([b])
+
+    def layer(self, i: int) -> wg_paged_kv:
+        """Layer i for the C entry points."""
+        return _cache(self.k[i], self.v[i], self.table, self.batch, self.k.get_device())

@@ -1,4 +1,4 @@
-"""Greedy speculative decoding (a 1.1B draft with config
+"""Speculative decoding, greedy or sampled (a 1.1B draft with config
 2's layout and the target's vocabulary proposes k = 4 tokens per step).
 
 The reference drafts on the host and verifies with forwardDraft / accept
@@ -81,7 +81,15 @@ def spec_sample(target: torch.Tensor, draft: torch.Tensor | None, drafts: torch.
 
 
 class SpeculativeDecoder:
-    def __init__(self, target: DecoderModel, draft: DecoderModel, k: int = 4, max_new: int = 512):
+    """temperature 0: greedy, as above. temperature > 0: the draft's tokens are
+    drawn from its own probabilities, kept against the target's, and the first
+    that is not kept is drawn again from what the target has left
+    (wg_spec_sample), so the emitted tokens are samples of the target whatever
+    the draft proposes. step() uses the random numbers u and u_draft as they
+    stand; run_step() has torch's generator of `seed` draw new ones before it."""
+
+    def __init__(self, target: DecoderModel, draft: DecoderModel, k: int = 4, max_new: int = 512,
+                 temperature: float = 0.0, seed: int = 0):
         if target.batch != draft.batch or target.cfg.vocab != draft.cfg.vocab:
             raise ValueError("target and draft must share batch and vocabulary")
         if target.max_rows < target.batch * (k + 1):
@@ -102,6 +110,17 @@ class SpeculativeDecoder:
         target.keep_prefixes(k + 1)
         draft.keep_prefixes(k + 1)
         self.graph = None
+        self.temperature = temperature
+        if temperature:
+            if target.world > 1 or draft.world > 1:
+                raise ValueError("sampled speculation needs the whole vocabulary on one GPU")
+            V = target.cfg.vocab
+            self.gen = torch.Generator(device="cuda")
+            self.gen.manual_seed(seed)
+            self.t_logits = torch.zeros((k + 1, B, V), device="cuda")
+            self.d_logits = torch.zeros((max(k, 1), B, V), device="cuda")
+            self.u = torch.zeros((B, k + 1), device="cuda")
+            self.u_draft = torch.zeros((max(k, 1), B, 1), device="cuda")
 
     def prefill(self, prompts: torch.Tensor):
         """Both models read the prompts; the first emitted token is the
@@ -110,9 +129,13 @@ class SpeculativeDecoder:
         self.d.prefill(prompts)
         self.out_len.zero_()
         self.accepted.zero_()
+        if self.temperature:
+            u = torch.rand((self.t.batch, 1), generator=self.gen, device="cuda")
+            spec_sample(self.t.logits, None, None, u, temperature=self.temperature, out=self.t.next_id.view(1, -1))
         self.out[:, 0].copy_(self.t.next_id)
         self.out_len.fill_(1)
         self.d.next_id.copy_(self.t.next_id)
+        self.draw()
 
     def step(self):
         """One draft-and-verify round (every sequence gains 1 .. k + 1 tokens)."""
@@ -124,20 +147,30 @@ class SpeculativeDecoder:
             self.pos_t0.copy_(t.pos)
         for j in range(k + 1):
             d.prefix_slot = j if d.has_conv else None
+            d.row_logits = self.d_logits[j:j + 1] if self.temperature and j < k else None
             try:
                 d.decode_step()
             finally:
                 d.prefix_slot = None
+                d.row_logits = None
             if j < k:
+                if self.temperature:
+                    spec_sample(self.d_logits[j], None, None, self.u_draft[j], temperature=self.temperature,
+                                out=d.next_id.view(1, -1))
                 self.drafts[:, j].copy_(d.next_id)
                 self.ver[:, j + 1].copy_(d.next_id)
         t.row_picks = self.picks
+        t.row_logits = self.t_logits if self.temperature else None
         t.prefix_slot = 0 if t.has_conv else None
         try:
             t.forward(self.ver.reshape(-1), t.batch * (k + 1))
         finally:
             t.row_picks = None
+            t.row_logits = None
             t.prefix_slot = None
+        if self.temperature:
+            spec_sample(self.t_logits, self.d_logits if k else None, self.drafts if k else None, self.u,
+                        temperature=self.temperature, out=self.picks)
         L = _lib.lib()
         t._c(L.wg_spec_accept(P(t.ctx.handle), P(self.drafts.data_ptr()), P(self.picks.data_ptr()), t.batch, k,
                               P(t.pos.data_ptr()), P(d.pos.data_ptr()), P(t.next_id.data_ptr()),
@@ -152,7 +185,14 @@ class SpeculativeDecoder:
         with torch.cuda.graph(self.graph):
             self.step()
 
+    def draw(self):
+        """New random numbers for the next round."""
+        if self.temperature:
+            self.u.uniform_(generator=self.gen)
+            self.u_draft.uniform_(generator=self.gen)
+
     def run_step(self):
+        self.draw()
         if self.graph is not None:
             self.graph.replay()
         else:
