@@ -54,14 +54,18 @@ __device__ __forceinline__ int row_seq(const PagedRows &a, int r, int lane) {
 
 // ---- append ----------------------------------------------------------------
 // A warp takes one row and up to `heads_per_warp` of its H + 2 Hkv heads: lane
-// l holds the rotate-half pairs (j, j + Dh/2) of a few neighbouring j, so that
-// a head is two coalesced loads and two coalesced stores, and the angles'
-// sines are made once for all the warp's heads. The angle of pair j at
-// position p, in turns, is p theta^(-2j/Dh) / 2 pi: its factor comes from the
-// host in 64 bits and the whole turns are taken off in 64 bits (one product,
-// one rounding, one difference), so that the fp32 sine sees an argument in
-// [-1, 1] half turns, exact at any position. Bound by its bytes for prompts
-// and by launch latency for decode rows.
+// l holds the rotate-half pairs (j, j + Dh/2) of four neighbouring j, so that a
+// head is two 16-byte loads and two 8-byte stores of Dh / 8 lanes, 1 to 4 heads
+// share a warp, 4 to 8 heads are in flight, and the row's sequence, page and
+// sines are found once for all the warp's heads, behind the first loads. The
+// angle of pair j at position p, in turns, is p theta^(-2j/Dh) / 2 pi: its
+// factor comes from the host in 64 bits and the whole turns are taken off in 64
+// bits (one product, one rounding, one difference), so that the fp32 sine sees
+// an argument in [-1, 1] half turns, exact at any position. Bound by its bytes
+// for prompts and by launch latency for decode rows: 16 sequences of up to 512
+// rows of 40 heads of 64 take 13.3 us, 4.6 TB/s with the ramps of one launch in
+// it (18.4 with 8-byte loads, 64-bit divisions and 8 heads a warp; 15.8 with the
+// 8 heads alone); 8 decode rows 2.4 us.
 
 struct RopeTurns {
   double t[128];  // theta^(-2j/Dh) / (2 pi)
@@ -75,22 +79,39 @@ __global__ void __launch_bounds__(256)
                       int heads_per_warp, int warps_per_row, unsigned *flags) {
   pdl_trigger();
   pdl_wait();
-  constexpr int kVec = Dh == 256 ? 4 : 2;          // neighbouring j a lane holds
-  constexpr int kLanes = Dh / 2 / kVec;            // lanes of a head (16 for Dh = 64: two heads at once)
-  constexpr int kHeads = 32 / kLanes;
+  constexpr int kLanes = Dh / 8, kHeads = 32 / kLanes;  // lanes of a head, heads at once
+  constexpr int kSets = Dh == 64 ? 2 : 4;                // times kHeads heads in flight
   const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int r = (int)(w / warps_per_row);
+  const unsigned w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);  // (the launcher keeps it in 32 bits)
+  const int r = (int)(w / (unsigned)warps_per_row);
   if (r >= pr.rows) return;
+  const int j0 = (lane % kLanes) * 4, sub = lane / kLanes;
+  const int NH = H + 2 * Hkv;
+  const int h0 = (int)(w - (unsigned)r * warps_per_row) * heads_per_warp, h1 = min(h0 + heads_per_warp, NH);
+  float x[kSets][4], y[kSets][4];  // dims j0 + i and j0 + i + Dh / 2
+  auto load = [&](int hh) {
+#pragma unroll
+    for (int e = 0; e < kSets; e++) {
+      const int h = hh + e * kHeads + sub;
+      float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
+      if (h < h1) {
+        const float *src = qkv + ((size_t)r * NH + h) * Dh + j0;
+        u = *reinterpret_cast<const float4 *>(src);
+        v = *reinterpret_cast<const float4 *>(src + Dh / 2);
+      }
+      x[e][0] = u.x, x[e][1] = u.y, x[e][2] = u.z, x[e][3] = u.w;
+      y[e][0] = v.x, y[e][1] = v.y, y[e][2] = v.z, y[e][3] = v.w;
+    }
+  };
+  load(h0);  // on its way while the row finds its sequence, page and angles
   const int b = row_seq(pr, r, lane);
   if (b < 0) return;
   int r0, n;
   seq_rows(pr, b, r0, n);
   const long long p = (long long)pr.pos[b] + (r - r0);
-  const int j0 = (lane % kLanes) * kVec, sub = lane / kLanes;
-  float cs[kVec], sn[kVec];
+  float cs[4], sn[4];
 #pragma unroll
-  for (int i = 0; i < kVec; i++) {
+  for (int i = 0; i < 4; i++) {
     const double t = (double)p * turns.t[j0 + i];
     sincospif((float)(2.0 * (t - rint(t))), &sn[i], &cs[i]);
   }
@@ -99,78 +120,62 @@ __global__ void __launch_bounds__(256)
   long long place = -1;
   if (p >= 0) {
     int page = -1;
-    if (p < cap) page = pt.table[(size_t)b * pt.max_pages + p / pt.page_size];
+    const unsigned slot = p < cap ? (unsigned)p / (unsigned)pt.page_size : 0;  // (cap fits an int)
+    if (p < cap) page = pt.table[(size_t)b * pt.max_pages + slot];
     if (page >= 0 && page < pt.num_pages)
-      place = page * (long long)page_stride + (p % pt.page_size) * (long long)row_stride;
+      place = page * (long long)page_stride + (int)((unsigned)p - slot * pt.page_size) * (long long)row_stride;
     else if (lane == 0)
       raise_flag(flags, kFlagBadArgument);
   }
-  const int NH = H + 2 * Hkv;
-  const int h0 = (int)(w - (long long)r * warps_per_row) * heads_per_warp;
   const float scale = rsqrtf((float)Dh);
-  for (int hh = h0; hh < min(h0 + heads_per_warp, NH); hh += kHeads) {
-    const int h = hh + sub;
-    const bool on = h < min(h0 + heads_per_warp, NH);
-    float x[kVec], y[kVec];  // dims j0 + i and j0 + i + Dh / 2
-    if (on) {
-      const float *src = qkv + ((size_t)r * NH + h) * Dh + j0;
-      if constexpr (kVec == 4) {
-        const float4 u = *reinterpret_cast<const float4 *>(src), v = *reinterpret_cast<const float4 *>(src + Dh / 2);
-        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-        y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
-      } else {
-        const float2 u = *reinterpret_cast<const float2 *>(src), v = *reinterpret_cast<const float2 *>(src + Dh / 2);
-        x[0] = u.x, x[1] = u.y;
-        y[0] = v.x, y[1] = v.y;
-      }
-    } else {
+  for (int hh = h0; hh < h1; hh += kSets * kHeads) {
+    if (hh > h0) load(hh);
 #pragma unroll
-      for (int i = 0; i < kVec; i++) x[i] = y[i] = 0.0f;
-    }
-    const bool is_q = h < H, is_v = h >= H + Hkv;
-    if (q_norm || k_norm) {  // the whole warp: a head's lanes sum its squares
-      float ss = 0.0f;
+    for (int e = 0; e < kSets; e++) {
+      const int h = hh + e * kHeads + sub;
+      if (hh + e * kHeads >= h1) break;
+      const bool is_q = h < H, is_v = h >= H + Hkv;
+      if (q_norm || k_norm) {  // the whole warp: a head's lanes sum its squares
+        float ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kVec; i++) ss += x[i] * x[i] + y[i] * y[i];
+        for (int i = 0; i < 4; i++) ss += x[e][i] * x[e][i] + y[e][i] * y[e][i];
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float *nw = is_q ? q_norm : is_v ? nullptr : k_norm;
-      if (nw && on) {
-        const float inv = rsqrtf(ss / (float)Dh + eps);
+        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float *nw = is_q ? q_norm : is_v ? nullptr : k_norm;
+        if (nw) {
+          const float inv = rsqrtf(ss / (float)Dh + eps);
 #pragma unroll
-        for (int i = 0; i < kVec; i++) {
-          x[i] *= inv * nw[j0 + i];
-          y[i] *= inv * nw[j0 + Dh / 2 + i];
+          for (int i = 0; i < 4; i++) {
+            x[e][i] *= inv * nw[j0 + i];
+            y[e][i] *= inv * nw[j0 + Dh / 2 + i];
+          }
         }
       }
-    }
-    if (!on) continue;
-    if (!is_v) {
-      const float sc = is_q ? scale : 1.0f;
+      if (h >= h1) continue;
+      if (!is_v) {
+        const float sc = is_q ? scale : 1.0f;
 #pragma unroll
-      for (int i = 0; i < kVec; i++) {
-        const float a = x[i], c = y[i];
-        x[i] = (a * cs[i] - c * sn[i]) * sc;
-        y[i] = (c * cs[i] + a * sn[i]) * sc;
+        for (int i = 0; i < 4; i++) {
+          const float a = x[e][i], c = y[e][i];
+          x[e][i] = (a * cs[i] - c * sn[i]) * sc;
+          y[e][i] = (c * cs[i] + a * sn[i]) * sc;
+        }
       }
-    }
-    T *dst;
-    if (is_q) {
-      dst = q_out + ((size_t)r * H + h) * Dh;
-      if (p < 0) {
+      T *dst;
+      if (is_q) {
+        dst = q_out + ((size_t)r * H + h) * Dh;
+        if (p < 0) {
 #pragma unroll
-        for (int i = 0; i < kVec; i++) x[i] = y[i] = 0.0f;
+          for (int i = 0; i < 4; i++) x[e][i] = y[e][i] = 0.0f;
+        }
+      } else {
+        if (place < 0) continue;
+        const int hk = is_v ? h - H - Hkv : h - H;
+        dst = (is_v ? v_pages : k_pages) + place + hk * head_stride;
       }
-    } else {
-      if (place < 0) continue;
-      const int hk = is_v ? h - H - Hkv : h - H;
-      dst = (is_v ? v_pages : k_pages) + place + hk * head_stride;
-    }
-    dst += j0;
-#pragma unroll
-    for (int i = 0; i < kVec; i += 2) {
-      *reinterpret_cast<uint32_t *>(dst + i) = pack2<T>(x[i], x[i + 1]);
-      *reinterpret_cast<uint32_t *>(dst + Dh / 2 + i) = pack2<T>(y[i], y[i + 1]);
+      dst += j0;
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(x[e][0], x[e][1]), pack2<T>(x[e][2], x[e][3]));
+      *reinterpret_cast<uint2 *>(dst + Dh / 2) = make_uint2(pack2<T>(y[e][0], y[e][1]), pack2<T>(y[e][2], y[e][3]));
     }
   }
 }
@@ -834,13 +839,14 @@ cudaError_t rope_t(const float *qkv, const PagedRows &pr, int H, int Hkv, const 
                    const float *k_norm, float eps, void *q_out, const wg_paged_kv &kv, unsigned *flags, int num_sms,
                    cudaStream_t s, bool pdl) {
   const int NH = H + 2 * Hkv;
-  // heads a warp takes: few rows, one (or the two that share a warp) for the
-  // shortest path; many, up to 8, which share the row's sines
-  const int least = Dh == 64 ? 2 : 1;
+  // heads a warp takes: few rows, those that share it at Dh / 8 lanes each, for
+  // the shortest path; many, up to 32, which share the row's sines
+  const int least = 256 / Dh;
   int hpw = least;
-  while (hpw < 8 && (long long)pr.rows * ((NH + hpw - 1) / hpw) > (long long)num_sms * 64) hpw *= 2;
+  while (hpw < 32 && (long long)pr.rows * ((NH + hpw - 1) / hpw) > (long long)num_sms * 64) hpw *= 2;
   const int wpr = (NH + hpw - 1) / hpw;
   const long long warps = (long long)pr.rows * wpr;
+  if (warps > 0xFFFFFF00LL) return cudaErrorInvalidValue;  // (a terabyte of heads)
   const PagedTable pt{kv.table, kv.max_pages, kv.num_pages, kv.page_size};
   const int64_t rs = stride_or(kv.row_stride, Dh), hs = stride_or(kv.head_stride, (int64_t)kv.page_size * Dh),
                 ps = stride_or(kv.page_stride, (int64_t)Hkv * kv.page_size * Dh);
