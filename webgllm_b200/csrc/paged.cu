@@ -767,68 +767,78 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
   }
 }
 
-// The sums of a unit that several CTAs share: block (c, row) joins row `row` of
-// the unit that begins in CTA c, its parts in CTA order. 512 threads: groups of
-// Dh / 4 threads take every n-th part.
+// The sums of a unit that several CTAs share: the blocks (c, .) join the rows of
+// the unit that begins in CTA c, each row's parts in CTA order. Dh / 4 threads
+// hold a row's dims; a unit of few parts has a group of them for each row, one of
+// many parts several groups a row, each of them every n-th part. Bound by the
+// latency of two dependent reads.
 constexpr int kJoinThreads = 512;
 
 template <typename T, int Dh>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const int *recs, const float *parts, int unit_rows,
                                                                   int H, int G, T *out) {
-  constexpr int kLanes = Dh / 4, kGroups = kJoinThreads / kLanes;
+  constexpr int kLanes = Dh / 4, kGroups = kJoinThreads / kLanes, kSpan = kLanes < 32 ? kLanes : 32;
   __shared__ float4 acc[kGroups][kLanes];
-  __shared__ float warp_m[kJoinThreads / 32], lsum[kGroups];
+  __shared__ float lsum[kGroups];
   pdl_trigger();
   pdl_wait();
   const int *rec = recs + blockIdx.x * 8;
   const int np = rec[0];
   if (np == 0) return;
-  const int slot = rec[1], r0 = rec[2], n = rec[3], hk = rec[4], m0 = rec[5], row = (int)blockIdx.y;
-  const int m = m0 + row, qi = m / G;
-  if (qi >= n) return;
+  const int slot = rec[1], r0 = rec[2], n = rec[3], hk = rec[4], m0 = rec[5];
   const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes;
+  int per_row = 1;  // groups of a row: two to four parts each
+  while (per_row < kGroups && per_row * 4 < np) per_row *= 2;
+  const int sub = grp % per_row, at_once = kGroups / per_row;
   const size_t stride = (size_t)unit_rows * (Dh + 2);
   // part j: the first in `slot`, then the first slots of the CTAs that follow
   auto part = [&](int j) { return parts + (j == 0 ? (size_t)slot : (size_t)2 * (blockIdx.x + j)) * stride; };
-  float mm = -INFINITY;
-  for (int j = tid; j < np; j += kJoinThreads) mm = fmaxf(mm, part(j)[row]);
+  const int rows = min((long long)unit_rows, (long long)n * G - m0);  // of the unit
+  for (int first = blockIdx.y * at_once; first < rows; first += gridDim.y * at_once) {
+    const int row = first + grp / per_row;
+    const bool on = row < rows;
+    float mm = -INFINITY, l = 0.0f;
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (on)
+      for (int j = tid % kSpan; j < np; j += kSpan) mm = fmaxf(mm, part(j)[row]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-  if ((tid & 31) == 0) warp_m[tid >> 5] = mm;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; i++) mm = fmaxf(mm, warp_m[i]);
-  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float l = 0.0f;
+    for (int o = kSpan / 2; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    if (on) {
 #pragma unroll 4
-  for (int j = grp; j < np; j += kGroups) {
-    const float *p = part(j);
-    const float f = mm == -INFINITY ? 0.0f : ex2(p[row] - mm);
-    const float4 v = *reinterpret_cast<const float4 *>(p + 2 * unit_rows + (size_t)row * Dh + lane * 4);
-    a.x += v.x * f;
-    a.y += v.y * f;
-    a.z += v.z * f;
-    a.w += v.w * f;
-    l += p[unit_rows + row] * f;
-  }
-  acc[grp][lane] = a;
-  if (lane == 0) lsum[grp] = l;
-  __syncthreads();
-  if (grp == 0) {
-#pragma unroll
-    for (int i = 1; i < kGroups; i++) {
-      const float4 v = acc[i][lane];
-      a.x += v.x;
-      a.y += v.y;
-      a.z += v.z;
-      a.w += v.w;
-      l += lsum[i];
+      for (int j = sub; j < np; j += per_row) {
+        const float *p = part(j);
+        const float f = mm == -INFINITY ? 0.0f : ex2(p[row] - mm);
+        const float4 v = *reinterpret_cast<const float4 *>(p + 2 * unit_rows + (size_t)row * Dh + lane * 4);
+        a.x += v.x * f;
+        a.y += v.y * f;
+        a.z += v.z * f;
+        a.w += v.w * f;
+        l += p[unit_rows + row] * f;
+      }
     }
-    const float inv = mm == -INFINITY ? 0.0f : 1.0f / l;
-    uint2 u;
-    u.x = pack2<T>(a.x * inv, a.y * inv);
-    u.y = pack2<T>(a.z * inv, a.w * inv);
-    *reinterpret_cast<uint2 *>(out + ((size_t)(r0 + qi) * H + hk * G + (m - qi * G)) * Dh + lane * 4) = u;
+    if (per_row > 1) {
+      acc[grp][lane] = a;
+      if (lane == 0) lsum[grp] = l;
+      __syncthreads();
+      if (sub == 0)
+        for (int i = 1; i < per_row; i++) {
+          const float4 v = acc[grp + i][lane];
+          a.x += v.x;
+          a.y += v.y;
+          a.z += v.z;
+          a.w += v.w;
+          l += lsum[grp + i];
+        }
+      __syncthreads();
+    }
+    if (on && sub == 0) {
+      const int m = m0 + row, qi = m / G;
+      const float inv = mm == -INFINITY ? 0.0f : 1.0f / l;
+      uint2 u;
+      u.x = pack2<T>(a.x * inv, a.y * inv);
+      u.y = pack2<T>(a.z * inv, a.w * inv);
+      *reinterpret_cast<uint2 *>(out + ((size_t)(r0 + qi) * H + hk * G + (m - qi * G)) * Dh + lane * 4) = u;
+    }
   }
 }
 
@@ -877,10 +887,14 @@ cudaError_t split_t(SplitArgs A, const wg_paged_kv &kv, void *workspace, int num
   A.part = reinterpret_cast<float *>(A.rec + (size_t)P * 8);
   e = launch_pdl(kern, dim3((unsigned)P), C::kThreads, C::kSmem, s, pdl, tk, tv, A);
   if (e != cudaSuccess) return e;
-  // rows of a unit that can exist: none past the longest sequence's
+  // blocks of a unit: one pass over the rows that can exist (none past the
+  // longest sequence's), with the groups a row that equal sequences would give
   const long long most = A.pr.row_start ? A.pr.rows : A.pr.rows / A.pr.batch;
-  const unsigned rows = (unsigned)(most * A.G < C::kRows ? most * A.G : C::kRows);
-  return launch_pdl(paged_join_kernel<T, Dh>, dim3((unsigned)P, rows), kJoinThreads, 0, s, pdl, A.rec, A.part,
+  const long long rows = most * A.G < C::kRows ? most * A.G : C::kRows, groups = kJoinThreads / (Dh / 4);
+  const long long parts = P / ((long long)A.pr.batch * A.Hkv) + 2;
+  const long long share = parts / 4 < groups ? (parts + 3) / 4 : groups;
+  const unsigned blocks = (unsigned)((rows * share + groups - 1) / groups);
+  return launch_pdl(paged_join_kernel<T, Dh>, dim3((unsigned)P, blocks), kJoinThreads, 0, s, pdl, A.rec, A.part,
                     C::kRows, A.H, A.G, reinterpret_cast<T *>(A.out));
 }
 
