@@ -63,7 +63,7 @@ int wg_paged_rope_kv(wg_ctx *ctx, const float *qkv, int rows, int batch, const i
  * window > 0 only those with j > p - window or j < sinks (a sliding window
  * and the first `sinks` positions, which stay visible). out = softmax(q . k)
  * v, a row that sees nothing gets zeros. q (scaled) and out [rows][H][Dh] in
- * the cache's dtype. Dh in {64, 128, 256}, H a multiple of Hkv, any rows per sequence
+ * the cache's dtype, not overlapping. Dh in {64, 128, 256}, H a multiple of Hkv, any rows per sequence
  * (one for a decode step, k + 1 to verify drafts, a prompt's chunk). What a
  * row does not see may hold anything, NaN included. A visible position whose
  * page entry names no page is left out and reported by wg_sync; positions

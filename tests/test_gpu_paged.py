@@ -451,6 +451,8 @@ def test_c_level_refusals():
                    (S, dict(most=1 << 28)), (S, dict(sp=4)), (S, dict(sh=-8)), (S, dict(sr=32)), (A, dict(rs=d + 1)),
                    (U, dict(rows=1 << 22, batch=1 << 20, most=1 << 20))]:
         assert attend(**kw) == st, kw
+    assert attend(out=d + 2 * 2 * 4 * 64 - 16) == A and "overlap" in L.wg_last_error(c.handle).decode()
+    assert attend(q=d + 16) == A and "overlap" in L.wg_last_error(c.handle).decode()
     for st, kw in [(A, dict(qkv=None)), (A, dict(qkv=d + 4)), (A, dict(theta=0.0)), (A, dict(theta=float("nan"))),
                    (A, dict(norm=d + 2)), (U, dict(rows=1 << 30, batch=1 << 20))]:
         assert append(**kw) == st, kw

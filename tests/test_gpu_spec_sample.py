@@ -59,6 +59,29 @@ def test_filtered_logits():
     assert torch.isfinite(t[n, b, got[n.cuda(), b.cuda()].long()]).all()
 
 
+@pytest.mark.parametrize("top", [3e5, 2e8, 1e12, 1e30, 3e38, -1e30])
+@pytest.mark.parametrize("T", [1.0, 1e-4])
+def test_logits_of_any_size(top, T):
+    """Finite logits however large: rows of three values, of which only the
+    largest has probability, and drafts that have it in the draft."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    B, k, V = 24, 2, 3001
+    values = sorted([top, top * (1 - 2.0 ** -10), -top])
+    values = torch.tensor(values, device="cuda")
+    t = values[torch.multinomial(torch.tensor([0.6, 0.1, 0.3], device="cuda").expand((k + 1) * B, 3), V,
+                                 replacement=True, generator=g)].view(k + 1, B, V)
+    d = values[torch.multinomial(torch.tensor([0.2, 0.1, 0.7], device="cuda").expand(k * B, 3), V,
+                                 replacement=True, generator=g)].view(k, B, V)
+    drafts = torch.multinomial((d == values[2]).float().view(k * B, V), 1, generator=g).view(k, B).t()
+    drafts = drafts.to(torch.int32).contiguous()
+    t[:, ::2].scatter_(2, drafts.t()[:, ::2, None].long().expand(k, B // 2, 1).contiguous(), top if top > 0 else -top)
+    u = torch.rand((B, k + 1), generator=g, device="cuda")
+    got = spec_sample(t, d, drafts, u, temperature=T)
+    wg.context().sync()
+    assert torch.equal(got.cpu(), R.spec_picks(t, d, drafts, u, T))
+
+
 def test_the_ends_of_u():
     """u = 0 accepts whatever has probability and draws the first token that
     has; the largest u below one draws a token that has."""

@@ -106,6 +106,9 @@ int wg_paged_attention(wg_ctx *ctx, const void *q, int rows, int batch, const in
   if (!q || !pos || !out || !workspace) return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_attention: null");
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(pos, 4) || !aligned(row_start, 4))
     return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_attention: misaligned tensor");
+  const long long bytes = (long long)rows * H * Dh * 2;
+  if ((const char *)q < (const char *)out + bytes && (const char *)out < (const char *)q + bytes)
+    return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_attention: q and out overlap");
   const size_t need = wg::paged_attention_workspace(Dh, ctx->num_sms);
   if (workspace_bytes < need)
     return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_attention: a workspace of %zu bytes, %zu needed", workspace_bytes,
