@@ -1,6 +1,7 @@
 """The paged cache's operators (include/webgllm_paged.h) against plain 64-bit
 forms (tests/paged_reference.py), within bounds derived from their arithmetic."""
 import ctypes
+import threading
 
 import pytest
 
@@ -12,7 +13,8 @@ if not torch.cuda.is_available():  # pragma: no cover
 
 import paged_reference as R  # noqa: E402
 import webgllm_b200 as wg  # noqa: E402
-from webgllm_b200 import _lib, paged  # noqa: E402
+from webgllm_b200 import _lib, paged, q4  # noqa: E402
+from webgllm_b200.speculative import spec_sample  # noqa: E402
 
 F16, BF16 = torch.float16, torch.bfloat16
 
@@ -476,3 +478,80 @@ def test_another_current_stream_is_honoured():
         out = run(q2, k, v, table, [1], [500])
     s.synchronize()
     assert torch.equal(out, want)
+
+
+def test_native_and_python_calls_agree(monkeypatch):
+    """The calls as one native step and through Python's code: the same bits;
+    what the native step does not take, it leaves alone."""
+    host = q4.host_calls()
+    if host is None:
+        pytest.skip("webgllm_b200._host is not built")
+    g = gen(4)
+    H, Hkv, Dh, page = 8, 2, 64, 16
+    q, k, v, table = make([2, 3], [50, 70], H, Hkv, Dh, page, BF16)
+    pos = torch.tensor([50, 70], dtype=torch.int32, device="cuda")
+    rs = starts([2, 3])
+    qkv = torch.randn((5, (H + 2 * Hkv) * Dh), generator=g, device="cuda")
+    norm = torch.rand(Dh, generator=g, device="cuda")
+    target = torch.randn((3, 4, 999), generator=g, device="cuda")
+    draft = torch.randn((2, 4, 999), generator=g, device="cuda")
+    drafts = torch.randint(0, 999, (4, 2), generator=g, device="cuda").to(torch.int32)
+    u = torch.rand((4, 3), generator=g, device="cuda")
+    ws = torch.empty(paged.workspace_bytes(0, Dh), dtype=torch.uint8, device="cuda")
+
+    def everything():
+        a = paged.rope_kv_paged(qkv, pos, k, v, table, heads=H, theta=1e6, q_norm=norm, eps=1e-6, row_start=rs)
+        b = paged.attention_paged(a, pos, k, v, table, window=40, sinks=2, row_start=rs)
+        c = paged.attention_paged(a, pos, k, v, table, row_start=rs, out=torch.empty_like(a), workspace=ws)
+        return [a, b, c, k.clone(), v.clone(), spec_sample(target, draft, drafts, u, temperature=0.5),
+                spec_sample(target[0], None, None, u[:, :1].contiguous())]
+
+    native = everything()
+    for name in ("webgllm_b200.paged", "webgllm_b200.speculative"):
+        monkeypatch.setattr(f"{name}.host_calls", lambda: None)
+    for x, y in zip(native, everything()):
+        assert x.dtype == y.dtype and torch.equal(x.view(torch.int16 if x.dtype == BF16 else x.dtype),
+                                                  y.view(torch.int16 if y.dtype == BF16 else y.dtype))
+    out = torch.empty_like(q)
+    assert host.attention_paged(q, pos, k, v, table, 0, 0, rs, out, None) is out
+    for bad in [(q[..., :32], pos, k, v, table, 0, 0, rs, None, None), (q, pos.long(), k, v, table, 0, 0, rs, None, None),
+                (q, pos, k, v[:, :, :8], table, 0, 0, rs, None, None), (q, pos, k, v, table, -1, 0, rs, None, None),
+                (q, pos, k, v, table, 1 << 40, 0, rs, None, None), (q, pos, k, v, table, 0, 0, pos, None, None),
+                (q, pos, k, v, table, 0, 0, rs, q, None), (q.cpu(), pos, k, v, table, 0, 0, rs, None, None),
+                (q, pos, k, v, table, 0, 0, rs, None, ws[:64]), (q, pos, k.float(), v, table, 0, 0, rs, None, None),
+                (q, pos, k, v, None, 0, 0, rs, None, None), (q, pos, k, v, table, 0, 0, rs, None), ()]:
+        assert host.attention_paged(*bad) is None
+    ctx = wg.context()
+    with ctx.lock:  # another thread's call: left to the Python code, which waits
+        assert host.attention_paged(q, pos, k, v, table, 0, 0, rs, None, None) is None
+    assert host.attention_paged(q, pos, k, v, table, 0, 0, rs, None, None) is not None and not ctx.lock.locked()
+    ctx.sync()
+
+
+def test_calls_from_several_threads():
+    """Threads on streams of their own: each call's work is on its thread's."""
+    H, Hkv, Dh, page = 8, 2, 64, 16
+    q, k, v, table = make([1] * 8, [300] * 8, H, Hkv, Dh, page, F16)
+    pos = torch.full((8,), 300, dtype=torch.int32, device="cuda")
+    want = paged.attention_paged(q, pos, k, v, table)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(200):
+                mine = q.clone()  # on this stream
+                out = paged.attention_paged(mine, pos, k, v, table)
+                mine.fill_(float("nan"))
+            s.synchronize()
+            if not torch.equal(out, want):
+                wrong.append(out)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    wg.context().sync()

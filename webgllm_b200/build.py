@@ -10,12 +10,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libwebgllm_b200.so"
+HOST = PKG / "_host.so"
 OBJ_DIR = PKG / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -42,9 +44,37 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def build_host(verbose: bool = False) -> Path | None:
+    """Compile csrc/host/ into the Python module _host.so against the installed
+    torch. None (and a line on stderr) where there is no torch to build with:
+    the calls then go through Python's code."""
+    srcs = sorted((CSRC / "host").glob("*.cpp"))
+    stamp = OBJ_DIR / "host_torch"
+    try:
+        import torch
+        from torch.utils.cpp_extension import CUDA_HOME, include_paths, library_paths
+    except ImportError as e:
+        print(f"{HOST.name} not built: {e}", file=sys.stderr)
+        return None
+    built_for = stamp.read_text() if stamp.exists() else ""
+    if built_for == torch.__version__ and not _stale(HOST, [*srcs, *(ROOT / "include").glob("*.h")]):
+        return HOST
+    includes = [*include_paths(), sysconfig.get_paths()["include"], str(Path(CUDA_HOME or "/usr/local/cuda") / "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes),
+           *map(str, srcs), "-o", str(HOST), *(f for p in library_paths() for f in (f"-L{p}", f"-Wl,-rpath,{p}")),
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    stamp.write_text(torch.__version__)
+    return HOST
+
+
 def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
     """Compile every .cu under csrc/ and link the shared library (rebuilds
-    only what changed; any header change rebuilds everything)."""
+    only what changed; any header change rebuilds everything), and the module
+    of host calls."""
     OBJ_DIR.mkdir(exist_ok=True)
     headers = list(CSRC.glob("*.cuh")) + list((ROOT / "include").glob("*.h"))
     objs = []
@@ -64,6 +94,7 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> Path:
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)
+    build_host(verbose)
     return LIB
 
 

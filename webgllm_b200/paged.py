@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import WG_BF16, WG_F16, GpuError, ShapeError, wg_paged_kv
-from .q4 import context
+from .q4 import context, host_calls
 
 __all__ = ["PagedCache", "attention_paged", "rope_kv_paged"]
 
@@ -81,6 +81,11 @@ def rope_kv_paged(qkv: torch.Tensor, pos: torch.Tensor, k: torch.Tensor, v: torc
     scaled queries [rows][heads][head dim] in the pages' dtype; keys and values
     go into the pages. Rows that belong to no sequence stay as they were in
     `out` (uninitialised in a new one)."""
+    host = host_calls()
+    if host is not None:
+        done = host.rope_kv_paged(qkv, pos, k, v, table, heads, theta, q_norm, k_norm, eps, row_start, out)
+        if done is not None:
+            return done
     batch, device = pos.numel(), k.get_device()
     kv = _cache(k, v, table, batch, device)
     _, hkv, _, dim = k.shape
@@ -126,6 +131,11 @@ def attention_paged(q: torch.Tensor, pos: torch.Tensor, k: torch.Tensor, v: torc
     and the first `sinks` positions. `workspace`: a uint8 tensor of
     workspace_bytes(...) that no overlapping call uses (default: a new one from
     torch's allocator, safe on any stream and inside a graph)."""
+    host = host_calls()
+    if host is not None:
+        done = host.attention_paged(q, pos, k, v, table, window, sinks, row_start, out, workspace)
+        if done is not None:
+            return done
     batch, device = pos.numel(), k.get_device()
     kv = _cache(k, v, table, batch, device)
     _, hkv, _, dim = k.shape

@@ -20,6 +20,7 @@ stream so that its work is ordered with the caller's.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 
 import numpy as np
@@ -160,6 +161,24 @@ def context(device: int | None = None) -> Context:
         if ctx is None:
             ctx = _contexts[device] = Context(device)
         return ctx
+
+
+@functools.cache
+def host_calls():
+    """webgllm_b200._host (csrc/host/calls.cpp: the checks and the call of the
+    serving operators as one native step) bound to the library, or None where
+    it is not built for this torch: the Python code then does the same, slower."""
+    try:
+        import torch  # noqa: F401  (its libraries)
+
+        from . import _host
+    except ImportError:
+        return None
+    L = _lib.lib()
+    _host.bind(_contexts, *(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+        L.wg_set_stream, L.wg_paged_rope_kv, L.wg_paged_attention, L.wg_paged_attention_workspace, L.wg_spec_sample,
+        L.wg_spec_sample_workspace)))
+    return _host
 
 
 class QuantMatrix:

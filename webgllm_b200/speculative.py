@@ -31,7 +31,7 @@ import torch
 
 from . import _lib
 from .model import DecoderConfig, DecoderModel
-from .q4 import context
+from .q4 import context, host_calls
 
 P = ctypes.c_void_p
 
@@ -49,6 +49,11 @@ def spec_sample(target: torch.Tensor, draft: torch.Tensor | None, drafts: torch.
     kept tokens, then the drawn one, then -1 (what wg_spec_accept takes).
     draft and drafts None (k = 0): one token per sequence drawn from target
     [1][batch][V] (or [batch][V])."""
+    host = host_calls()
+    if host is not None:
+        done = host.spec_sample(target, draft, drafts, u, temperature, out)
+        if done is not None:
+            return done
     if target.dim() == 2 and draft is None:
         target = target.unsqueeze(0)
     device = target.get_device()
