@@ -154,6 +154,25 @@ def test_rows_without_probabilities_are_reported(bad, V):
     assert torch.equal(got.cpu()[:, ok], R.spec_picks(t[:, ok], d[:, ok], drafts[ok], u[ok], 1.0))
 
 
+@pytest.mark.parametrize("bad", ["nan", "inf", "none"])
+@pytest.mark.parametrize("V", [1, 9, 3000, 40000, 128256])
+def test_plain_sampling_of_rows_without_probabilities(bad, V):
+    t, _, _, u = make(5, 0, V, 0.0, seed=2)
+    if bad == "nan":
+        t[0, 3, V // 3] = float("nan")
+    elif bad == "inf":
+        t[0, 3, V - 1] = float("inf")
+    else:
+        t[0, 3] = -float("inf")
+    t[0, 1, V // 2:] = -float("inf") if V > 1 else 0.0
+    got = spec_sample(t, None, None, u)
+    with pytest.raises(wg.GpuError):
+        wg.context().sync()
+    assert ((got >= 0) & (got < V)).all()
+    ok = [0, 1, 2, 4]
+    assert torch.equal(got.cpu()[:, ok], R.spec_picks(t[:, ok], None, None, u[ok], 1.0))
+
+
 def test_unaligned_rows_and_views():
     """Logits that start at any float (an odd vocabulary, a view)."""
     for off in range(4):
