@@ -221,6 +221,7 @@ struct SplitArgs {
   int window, sinks;
   int box_rows;  // keys of one TMA box: divides page_size and the tile
   int stages;
+  int whole;     // units are not split: a CTA takes whole ones
   int *rec;      // workspace: [P][8]
   float *part;   // workspace: [2 P][rows * (Dh + 2)]
   unsigned *flags;
@@ -267,6 +268,7 @@ struct SplitCfg {
   static constexpr int KW = Dh == 64 ? 32 : 16;    // keys of a warp
   static constexpr int kKeys = 4 * KW;             // of a tile
   static constexpr int kRows = 16 * MT;
+  static constexpr int kWhole = Dh == 256 ? 3 : 4;  // tiles up to which a unit is not split
   static constexpr int kWarps = 4 * MT;            // consumers
   static constexpr int kThreads = (kWarps + 1) * 32;
   static constexpr int kCtas = MT == 1 && Dh <= 128 ? 2 : 1;  // per SM
@@ -335,14 +337,14 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
   // up to 32 sequences, else by the CTA, in passes of a thread a sequence
   int total = 0, b = A.pr.batch, base = 0, per, start, end;
   auto share = [&]() {
-    per = max((total + P - 1) / P, max(1, kMinKeys / kKeys));
+    per = max((total + P - 1) / P, A.whole ? 1 : max(1, kMinKeys / kKeys));
     start = (int)min((long long)total, (long long)cta * per);
     end = (int)min((long long)total, (long long)start + per);
   };
   auto work_of = [&](int i) {
     if (i >= A.pr.batch) return 0;
     const SeqWork w = seq_work(A, i, C::kRows, kKeys);
-    return A.Hkv * w.mt * w.nt;
+    return A.Hkv * w.mt * (A.whole ? 1 : w.nt);
   };
   if (A.pr.batch <= 32) {
     const int v = work_of(lane);
@@ -404,14 +406,14 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
     const int groups = A.box_rows / 16, gmask = (1 << groups) - 1;
     for (int pos = start; pos < end;) {
       const SeqWork w = seq_work(A, b, C::kRows, kKeys);
-      const int work = A.Hkv * w.mt * w.nt;
+      const int steps = A.whole ? 1 : w.nt, work = A.Hkv * w.mt * steps;
       if (pos >= base + work) {
         base += work;
         b++;
         continue;
       }
-      const int unit = (pos - base) / w.nt, t0 = (pos - base) - unit * w.nt;
-      const int t1 = min(w.nt, t0 + (end - pos));
+      const int unit = (pos - base) / steps, t0 = (pos - base) - unit * steps;
+      const int t1 = A.whole ? w.nt : min(w.nt, t0 + (end - pos));
       const int hk = unit / w.mt;
       const int32_t *row = A.pt.table + (size_t)b * A.pt.max_pages;
       // the box's page entry and whether any row sees a key of it
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
         seen = seen_next;
         advance();
       }
-      pos += t1 - t0;
+      pos += A.whole ? 1 : t1 - t0;
     }
     // after a wait that ran out, no copy may still be on its way into this
     // CTA's memory when it exits
@@ -464,14 +466,14 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
     int rec[5] = {0, 0, 0, 0, 0};
     for (int pos = start; pos < end;) {
       const SeqWork w = seq_work(A, b, C::kRows, kKeys);
-      const int work = A.Hkv * w.mt * w.nt;
+      const int steps = A.whole ? 1 : w.nt, work = A.Hkv * w.mt * steps;
       if (pos >= base + work) {
         base += work;
         b++;
         continue;
       }
-      const int unit = (pos - base) / w.nt, t0 = (pos - base) - unit * w.nt;
-      const int t1 = min(w.nt, t0 + (end - pos));
+      const int unit = (pos - base) / steps, t0 = (pos - base) - unit * steps;
+      const int t1 = A.whole ? w.nt : min(w.nt, t0 + (end - pos));
       const int hk = unit / w.mt, m0 = (unit - hk * w.mt) * C::kRows;
 
       // queries, 16 bytes a load, through the merge buffer into A fragments; the
@@ -756,7 +758,7 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
         rec[4] = m0;
       }
       sync();  // red and sm_m / sm_l are free again
-      pos += t1 - t0;
+      pos += A.whole ? 1 : t1 - t0;
     }
     if (tid == 0) {
       int *r = A.rec + cta * 8;
@@ -881,12 +883,20 @@ cudaError_t split_t(SplitArgs A, const wg_paged_kv &kv, void *workspace, int num
   // CTAs: no more than there can be work for
   const long long units = (((long long)A.pr.rows * A.G + C::kRows - 1) / C::kRows + A.pr.batch) * A.Hkv;
   const long long keys = (long long)kv.max_pages * kv.page_size;
-  const long long work = units * ((keys + kMinKeys - 1) / kMinKeys);
+  // Few keys that a row can see (by the table's width and the window, what the
+  // host knows): whole units, and no second launch to join their parts (one
+  // sequence, Dh = 64, 4 KV heads: 256 keys 5.8 us for 7.6, 384 7.1 for 8.1, 512
+  // 8.3 for 8.1; Dh = 128, 8 KV heads: 128 keys 6.8 for 8.6, 256 9.0 for 9.3; Dh =
+  // 256: 128 keys 9.0 for 10.2, 192 10.8 for 10.7; and a launch less on the host)
+  const long long rows_seq = A.pr.row_start ? A.pr.rows : A.pr.rows / A.pr.batch;
+  const long long seen = A.window ? (long long)A.window + A.sinks + rows_seq + 2 * C::kKeys : keys;
+  A.whole = (seen < keys ? seen : keys) <= C::kWhole * C::kKeys;
+  const long long work = A.whole ? units : units * ((keys + kMinKeys - 1) / kMinKeys);
   const int P = (int)(work < num_sms * C::kCtas ? work : num_sms * C::kCtas);
   A.rec = reinterpret_cast<int *>(workspace);
   A.part = reinterpret_cast<float *>(A.rec + (size_t)P * 8);
   e = launch_pdl(kern, dim3((unsigned)P), C::kThreads, C::kSmem, s, pdl, tk, tv, A);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || A.whole) return e;
   // blocks of a unit: one pass over the rows that can exist (none past the
   // longest sequence's), with the groups a row that equal sequences would give
   const long long most = A.pr.row_start ? A.pr.rows : A.pr.rows / A.pr.batch;
