@@ -53,7 +53,7 @@ __device__ __forceinline__ int row_seq(const PagedRows &a, int r, int lane) {
 }
 
 // ---- append ----------------------------------------------------------------
-// A warp takes one row and up to `heads_per_warp` of its H + 2 Hkv heads: lane
+// A warp takes one row and up to `heads_per_warp` (16) of its H + 2 Hkv heads: lane
 // l holds the rotate-half pairs (j, j + Dh/2) of four neighbouring j, so that a
 // head is two 16-byte loads and two 8-byte stores of Dh / 8 lanes, 1 to 4 heads
 // share a warp, 4 to 8 heads are in flight, and the row's sequence, page and
@@ -63,16 +63,16 @@ __device__ __forceinline__ int row_seq(const PagedRows &a, int r, int lane) {
 // bits (one product, one rounding, one difference), so that the fp32 sine sees
 // an argument in [-1, 1] half turns, exact at any position. Bound by its bytes
 // for prompts and by launch latency for decode rows: 16 sequences of up to 512
-// rows of 40 heads of 64 take 13.3 us, 4.6 TB/s with the ramps of one launch in
-// it (18.4 with 8-byte loads, 64-bit divisions and 8 heads a warp; 15.8 with the
-// 8 heads alone); 8 decode rows 2.4 us.
+// rows of 40 heads of 64 take 14.9 us from HBM, 4.1 TB/s with the ramps of one
+// launch in it (17.5 in blocks of 256 threads, 32 heads a warp and with loads that
+// stay in L2, 15.7 with 8 heads a warp); 8 decode rows 2.5 us.
 
 struct RopeTurns {
   double t[128];  // theta^(-2j/Dh) / (2 pi)
 };
 
 template <typename T, int Dh>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(64)
     paged_rope_kernel(const float *qkv, const PagedRows pr, int H, int Hkv, const RopeTurns turns,
                       const float *q_norm, const float *k_norm, float eps, T *q_out, T *k_pages, T *v_pages,
                       int64_t page_stride, int64_t head_stride, int64_t row_stride, const PagedTable pt,
@@ -96,8 +96,8 @@ __global__ void __launch_bounds__(256)
       float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
       if (h < h1) {
         const float *src = qkv + ((size_t)r * NH + h) * Dh + j0;
-        u = *reinterpret_cast<const float4 *>(src);
-        v = *reinterpret_cast<const float4 *>(src + Dh / 2);
+        u = __ldcs(reinterpret_cast<const float4 *>(src));  // read once
+        v = __ldcs(reinterpret_cast<const float4 *>(src + Dh / 2));
       }
       x[e][0] = u.x, x[e][1] = u.y, x[e][2] = u.z, x[e][3] = u.w;
       y[e][0] = v.x, y[e][1] = v.y, y[e][2] = v.z, y[e][3] = v.w;
@@ -852,17 +852,17 @@ cudaError_t rope_t(const float *qkv, const PagedRows &pr, int H, int Hkv, const 
                    cudaStream_t s, bool pdl) {
   const int NH = H + 2 * Hkv;
   // heads a warp takes: few rows, those that share it at Dh / 8 lanes each, for
-  // the shortest path; many, up to 32, which share the row's sines
+  // the shortest path; many, up to 16, which share the row's sines
   const int least = 256 / Dh;
   int hpw = least;
-  while (hpw < 32 && (long long)pr.rows * ((NH + hpw - 1) / hpw) > (long long)num_sms * 64) hpw *= 2;
+  while (hpw < 16 && (long long)pr.rows * ((NH + hpw - 1) / hpw) > (long long)num_sms * 64) hpw *= 2;
   const int wpr = (NH + hpw - 1) / hpw;
   const long long warps = (long long)pr.rows * wpr;
   if (warps > 0xFFFFFF00LL) return cudaErrorInvalidValue;  // (a terabyte of heads)
   const PagedTable pt{kv.table, kv.max_pages, kv.num_pages, kv.page_size};
   const int64_t rs = stride_or(kv.row_stride, Dh), hs = stride_or(kv.head_stride, (int64_t)kv.page_size * Dh),
                 ps = stride_or(kv.page_stride, (int64_t)Hkv * kv.page_size * Dh);
-  const int threads = warps <= num_sms * 4 ? 64 : 256;
+  constexpr int threads = 64;
   const unsigned blocks = (unsigned)((warps * 32 + threads - 1) / threads);
   return launch_pdl(paged_rope_kernel<T, Dh>, dim3(blocks), threads, 0, s, pdl, qkv, pr, H, Hkv, turns, q_norm, k_norm, eps,
                 reinterpret_cast<T *>(q_out), reinterpret_cast<T *>(kv.k), reinterpret_cast<T *>(kv.v), ps, hs, rs, pt,
