@@ -7,7 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import webgllm_b200 as wg  # noqa: E402
-from webgllm_b200 import _lib, paged  # noqa: E402
+from webgllm_b200 import _lib, paged, q4  # noqa: E402
 from webgllm_b200.speculative import spec_sample  # noqa: E402
 
 
@@ -98,3 +98,19 @@ def test_cache_refusals():
         paged.PagedCache(1, 1, 1, 64, 4, 64, dtype=torch.float32, device="cpu")
     with pytest.raises(wg.RangeError):
         cache().reserve(0, 113)
+
+
+def test_native_calls_leave_what_they_do_not_take():
+    """webgllm_b200._host takes CUDA tensors only; for anything else it returns
+    None and Python's code says what is wrong."""
+    host = q4.host_calls()
+    if host is None:
+        pytest.skip("webgllm_b200._host is not built")
+    t = torch.zeros(2, 4, 16, 64, dtype=torch.float16)
+    i = torch.zeros(2, dtype=torch.int32)
+    table = torch.zeros((2, 3), dtype=torch.int32)
+    assert host.attention_paged(t[:, 0], i, t, t, table, 0, 0, None, None, None) is None
+    assert host.rope_kv_paged(t, i, t, t, table, 4, 1e4, None, None, 1e-5, None, None) is None
+    assert host.spec_sample(torch.zeros(1, 2, 8), None, None, torch.zeros(2, 1), 1.0, None) is None
+    for fn in (host.attention_paged, host.rope_kv_paged, host.spec_sample):
+        assert fn() is None and fn(*[None] * 10) is None and fn(*["x"] * 12) is None and fn(*[object()] * 6) is None

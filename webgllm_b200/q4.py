@@ -172,9 +172,10 @@ def host_calls():
         import torch  # noqa: F401  (its libraries)
 
         from . import _host
+
+        L = _lib.lib()
     except ImportError:
         return None
-    L = _lib.lib()
     _host.bind(_contexts, *(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
         L.wg_set_stream, L.wg_paged_rope_kv, L.wg_paged_attention, L.wg_paged_attention_workspace, L.wg_spec_sample,
         L.wg_spec_sample_workspace)))

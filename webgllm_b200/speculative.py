@@ -1,5 +1,6 @@
-"""Speculative decoding, greedy or sampled (a 1.1B draft with config
-2's layout and the target's vocabulary proposes k = 4 tokens per step).
+"""Speculative decoding, greedy or sampled (for the 8B shape: a 1.1B draft with
+the 1.1B model's layout and the target's vocabulary proposes k = 4 tokens per
+step).
 
 The reference drafts on the host and verifies with forwardDraft / accept
 (packages/webgllm/src/engine.ts:8035,8063). Here one step stays on the GPU
