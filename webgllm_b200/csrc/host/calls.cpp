@@ -87,11 +87,13 @@ at::Tensor make(at::IntArrayRef shape, at::ScalarType type, int device) {
 // here (no context yet, another current device, the lock is another thread's).
 struct Held {
   wg_ctx *ctx = nullptr;
-  PyObject *lock = nullptr;
+  PyObject *owner = nullptr, *lock = nullptr;  // kept while other threads run
   void *stream = nullptr;
 
   explicit Held(int device) {
     if (!contexts_ || c10::cuda::current_device() != device) return;
+    const cudaStream_t s = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    stream = s ? s : cudaStreamLegacy;
     PyObject *key = PyLong_FromLong(device);
     PyObject *c = key ? PyDict_GetItemWithError(contexts_, key) : nullptr;  // borrowed
     Py_XDECREF(key);
@@ -99,6 +101,7 @@ struct Held {
     PyObject *got = mine ? PyObject_CallMethodOneArg(mine, s_acquire_, Py_False) : nullptr;
     if (got == Py_True) {
       lock = mine;
+      owner = Py_NewRef(c);
       PyObject *h = PyObject_GetAttr(c, s_handle_);
       if (h && h != Py_None) ctx = static_cast<wg_ctx *>(PyLong_AsVoidPtr(h));
       Py_XDECREF(h);
@@ -107,14 +110,13 @@ struct Held {
     }
     Py_XDECREF(got);
     PyErr_Clear();
-    const cudaStream_t s = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
-    stream = s ? s : cudaStreamLegacy;
   }
   ~Held() {
     if (!lock) return;
     PyObject *r = PyObject_CallMethodNoArgs(lock, s_release_);
     Py_XDECREF(r);
     Py_DECREF(lock);
+    Py_DECREF(owner);
   }
   Held(const Held &) = delete;
   Held &operator=(const Held &) = delete;
