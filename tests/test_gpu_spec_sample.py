@@ -173,6 +173,37 @@ def test_plain_sampling_of_rows_without_probabilities(bad, V):
     assert torch.equal(got.cpu()[:, ok], R.spec_picks(t[:, ok], None, None, u[ok], 1.0))
 
 
+@pytest.mark.parametrize("V,k", [(32000, 0), (128256, 0), (128256, 1)])
+def test_slices_without_weight_and_a_draw_on_their_border(V, k):
+    """Runs of the vocabulary with the contents A B C none C B A none: u = 0.5
+    draws on the border between the two C, whose running sum comes out an ulp
+    higher or lower next to the run without weight, by the order of its additions.
+    Each row gets one pick all the same: a neighbour of the border, or where the
+    sum rounds past it, and the same one every time."""
+    runs = {32000: 8, 128256: 16}[V]  # as many as CTAs share a row
+    n = -(-V // runs)
+    B = 18 if V > 32000 else 64
+    g = torch.Generator(device="cuda")
+    g.manual_seed(V + k)
+    none = torch.full((B, n), -float("inf"), device="cuda")
+    a, b, c = (none.clone().index_copy_(1, torch.tensor([i], device="cuda"), torch.randn((B, 1), generator=g, device="cuda"))
+               for i in (3, n // 2, n - 200))
+    row = torch.cat([a, b, c, none, c, b, a, none] + [none] * (runs - 8), 1)[:, :V]
+    want = {2 * n + n - 200, 4 * n + n - 200}  # the two C
+    t = row.expand(k + 1, B, V).contiguous()
+    u = torch.full((B, k + 1), 0.5, device="cuda")
+    d = drafts = None
+    if k:  # a draft that the target keeps: the token is drawn from the last row
+        d = torch.zeros((k, B, V), device="cuda")
+        drafts = torch.full((B, k), 3, dtype=torch.int32, device="cuda")
+    out = torch.full((k + 1, B), -7, dtype=torch.int32, device="cuda")
+    spec_sample(t, d, drafts, u, out=out)
+    wg.context().sync()
+    assert set(out[k].tolist()) <= want
+    for _ in range(5):
+        assert torch.equal(spec_sample(t, d, drafts, u), out)
+
+
 def test_unaligned_rows_and_views():
     """Logits that start at any float (an odd vocabulary, a view)."""
     for off in range(4):

@@ -96,12 +96,17 @@ __device__ __forceinline__ double cta_sum(double v, double *warp_part) {
   return last16(scan16((lane & 15) < kWarps ? warp_part[lane & 15] : 0.0, lane));
 }
 
-// The running sums of the cluster's CTAs (their *mine), the same bits in every
-// CTA: rank i's share is [incl(i - 1), incl(i)). Needs a cluster barrier
+// The cluster's CTAs' values (their *mine) in lanes 0 .. 15 and again in 16 .. 31,
+// and their running sums, the same bits in every CTA. The sums of neighbouring
+// lanes are added in different orders: next to a CTA without weight they may fall
+// or rise by their last bit, so they order no shares. Needs a cluster barrier
 // between the writes and the call.
-__device__ __forceinline__ double ranks_scan(const double *mine, int lane, int CL) {
+__device__ __forceinline__ double rank_value(const double *mine, int lane, int CL) {
   const int i = lane & 15;
-  return scan16(i < CL ? *cg::this_cluster().map_shared_rank(mine, i) : 0.0, lane);
+  return i < CL ? *cg::this_cluster().map_shared_rank(mine, i) : 0.0;
+}
+__device__ __forceinline__ double ranks_scan(const double *mine, int lane, int CL) {
+  return scan16(rank_value(mine, lane, CL), lane);
 }
 // exp((x - max) / T) in 64 bits, off by less than 2^-47: 2^(n / 16) from a
 // table (16 doubles in shared memory: one bank row, no conflicts whatever the
@@ -423,7 +428,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) spec_sample_kernel(co
   };
 
   // ---- (4) the token: the first whose running sum exceeds u times the total
-  double total, before, after, warp_total, warp_head;
+  double total, rank_head, warp_total, warp_head;  // (rank_head: lane i's of CTA i)
   const int per_slot = (per_warp / 256 + kSlots - 1) / kSlots * 256;  // rounds that share a slot
   for (;;) {
     warp_total = 0.0;
@@ -446,11 +451,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) spec_sample_kernel(co
     warp_head = warp > 0 ? __shfl_sync(0xffffffffu, warps, warp - 1) : 0.0;
     if (tid == 15) cta_part[3] = warps;
     cl.sync();
-    const double ranks = ranks_scan(&cta_part[3], lane, CL);
+    const double mass = rank_value(&cta_part[3], lane, CL), ranks = scan16(mass, lane);
     total = last16(ranks);
-    after = __shfl_sync(0xffffffffu, ranks, rank);
-    before = __shfl_sync(0xffffffffu, ranks, rank ? rank - 1 : 0);
-    if (!rank) before = 0.0;
+    rank_head = __shfl_up_sync(0xffffffffu, ranks, 1, 16);
+    if (!(lane & 15)) rank_head = 0.0;
+    if (!(mass > 0.0)) rank_head = INFINITY;
     // p and q may agree to the last bit everywhere: then the rejected token's
     // place goes to another token of p
     if (!diff || without || total > 0.0) break;
@@ -462,12 +467,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) spec_sample_kernel(co
   if (!(u > 0.0)) u = 0.0;
   const double goal = u * total;
   if (!(total > 0.0)) report();  // all of p on the rejected token: q was no distribution
-  // One CTA holds the goal. There: the last warp that has weight and whose head
-  // is not past the goal, in it the last round, there the last run of 32, and in
+  // The last CTA that has weight and whose head is not past the goal (the first
+  // that has weight has head 0, so there is always one, the same in every CTA),
+  // in it the last such warp, there the last round, the last run of 32, and in
   // that the first token past the goal. (Where rounding leaves the goal past the
   // run's own sum: its last token with weight.)
-  if (total > 0.0 && before <= goal && goal < after) {
-    double head = before + warp_head;
+  const unsigned ranks_at = __ballot_sync(0xffffffffu, lane < 16 && rank_head <= goal);
+  if (total > 0.0 && 31 - __clz(ranks_at) == rank) {
+    double head = __shfl_sync(0xffffffffu, rank_head, rank) + warp_head;
     if (lane == 0 && warp_total > 0.0 && head <= goal) atomicMax(&s_owner, warp);
     __syncthreads();
     if (warp == s_owner) {
