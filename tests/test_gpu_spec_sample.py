@@ -204,6 +204,52 @@ def test_slices_without_weight_and_a_draw_on_their_border(V, k):
         assert torch.equal(spec_sample(t, d, drafts, u), out)
 
 
+def test_draws_beside_a_border_of_nearly_equal_distributions():
+    """Draft and target differ by a millionth (the draft's logits all higher by
+    some amount, which changes nothing), so that p - q cancels all but the last
+    third of a double: weights good to 2^-47 leave the border between two tokens
+    of the residual within 4e-8 of its place in u (2^-47 of a weight over a
+    residual of at least 2e-7 of it), and 2.5e-7 beside it (two to four steps of
+    u) the pick is decided."""
+    B = 8192
+    g = torch.Generator(device="cuda")
+    g.manual_seed(12)
+    t = 2.0 * torch.randn((2, B, 3), generator=g, device="cuda")
+    d = t[:1] + 4.0 * torch.rand((1, B, 1), generator=g, device="cuda")
+    d[..., 2] += 4e-6  # the draft's token, a hair likelier than in the target: rejected by u_0, residual on 0 and 1
+    p, q = torch.softmax(t[0].double(), 1), torch.softmax(d[0].double(), 1)
+    r = (p - q)[:, :2]
+    top = 1.0 - 2.0 ** -24
+    use = (r > 2e-7 * p[:, :2]).all(1) & (top * q[:, 2] >= p[:, 2] * (1 + 1e-9))
+    border = r[:, 0] / r.sum(1)
+    use &= (border > 0.01) & (border < 0.99)
+    assert use.sum() > 1000
+    side = torch.arange(B, device="cuda") % 2  # below or above the border
+    u = torch.stack([torch.full((B,), top, dtype=torch.float64, device="cuda"), border + (side * 2 - 1) * 2.5e-7], 1).float()
+    drafts = torch.full((B, 1), 2, dtype=torch.int32, device="cuda")
+    got = spec_sample(t, d, drafts, u)
+    wg.context().sync()
+    assert torch.equal(got[0][use].long(), side[use])
+
+
+def test_hidden_logits_have_no_weight_at_any_maximum():
+    """-inf beside one token, at every size of its logit and down to the lowest
+    temperatures: that token is drawn."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    B, V = 2000, 70
+    top = (torch.rand(B, generator=g, device="cuda") * 2 - 1) * 5000
+    top[0] = 4897.20654
+    at = torch.randint(0, V, (B,), generator=g, device="cuda")
+    t = torch.full((1, B, V), -float("inf"), device="cuda")
+    t[0, torch.arange(B, device="cuda"), at] = top
+    for T in (1e-4, 0.001, 0.37, 1.0):
+        u = torch.rand((B, 1), generator=g, device="cuda")
+        got = spec_sample(t, None, None, u, temperature=T)
+        wg.context().sync()
+        assert torch.equal(got[0].long(), at)
+
+
 def test_unaligned_rows_and_views():
     """Logits that start at any float (an odd vocabulary, a view)."""
     for off in range(4):

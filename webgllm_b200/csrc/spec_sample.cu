@@ -108,23 +108,28 @@ __device__ __forceinline__ double rank_value(const double *mine, int lane, int C
 __device__ __forceinline__ double ranks_scan(const double *mine, int lane, int CL) {
   return scan16(rank_value(mine, lane, CL), lane);
 }
-// exp((x - max) / T) in 64 bits, off by less than 2^-47: 2^(n / 16) from a
-// table (16 doubles in shared memory: one bank row, no conflicts whatever the
-// lanes pick), n the nearest to 16 log2 e (x - max) / T, times the polynomial of
+// exp((x - ref) / T) in 64 bits, off by less than 2^-47: with y = 16 log2 e x / T
+// - whole, 2^(n / 16) from a table (16 doubles in shared memory: one bank row, no
+// conflicts whatever the lanes pick), n the nearest to y, times the polynomial of
 // degree 5 through 2^(f / 16) at the six Chebyshev points of |f| <= 1/2 (off by
-// 4.6e-15). Ten 64-bit operations and no branch: the 64-bit pipe (a warp's
-// operation every 2.8 cycles) bounds these passes. Below 2^-990 and at -inf: 0.
+// 4.6e-15). `whole` is the whole number at or below 16 log2 e max / T, so ref is
+// at most 1/16 octave below the maximum and weights reach 2^(1/16). It has to be
+// whole: next to the rounding constant a fraction would be lost, and |f| with it
+// reach 1, where the polynomial is off by 6e-12. Ten 64-bit operations and no
+// branch: the 64-bit pipe (a warp's operation every 2.8 cycles) bounds these
+// passes. Below 2^-990 and at -inf: 0.
 __constant__ double kRoots[16] = {
     1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
     1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
     1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
     1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
 struct Exp64 {
-  double scale, shift;  // 16 log2 e / T, and - max times it
+  double scale, shift;  // 16 log2 e / T, and -whole
   float low, max;       // logits at or below `low` have weight 0
   const double *table;
   __device__ __forceinline__ double operator()(float x) const {
-    // (a hidden logit as the maximum, times the table's 17th entry, 0)
+    // (a hidden logit as the maximum, whose n is 0 or 1, times the table's 17th
+    // entry, 0: its exponent must not be lowered)
     const bool some = x > low;
     const double xd = (double)(some ? x : max);
     const double t = fma(xd, scale, shift + 6755399441055744.0);  // n in the low bits
@@ -262,8 +267,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) spec_sample_kernel(co
     // A maximum so large that its neighbours in fp32 lie below 2^-990 (where the
     // product with the scale would lose its last bits): weights 1 and 0.
     if (fabs(m * a.scale) > 1e12) return Exp64{0.0, 0.0, nextafterf(row_m[r], -INFINITY), row_m[r], table};
-    return Exp64{a.scale, -m * a.scale, low > -3.4e38 ? (float)low : -3.4e38f, row_m[r], table};
+    return Exp64{a.scale, -floor(m * a.scale), low > -3.4e38 ? (float)low : -3.4e38f, row_m[r], table};
   };
+  // a row's sum from its pieces (over the maximum), as one of weights(r)
+  auto sum_of = [&](int r, const Exp64 &w) { return row_z[r] * w(row_m[r]); };
   auto round_of = [&](const float *x, int i0, float v[8]) {
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] = i0 + 32 * e < w1 ? __ldg(x + i0 + 32 * e) : -INFINITY;
@@ -322,8 +329,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) spec_sample_kernel(co
     if (warp == kWarps - 1) {
       bool kept_it = false, close = false;
       if (lane < k && d >= 0 && d < V) {
-        const double lhs = u_d * weights(k + 1 + lane)(xq_d) * row_z[lane];
-        const double rhs = weights(lane)(xp_d) * row_z[k + 1 + lane];
+        const Exp64 wp = weights(lane), wq = weights(k + 1 + lane);
+        const double lhs = u_d * wq(xq_d) * sum_of(lane, wp), rhs = wp(xp_d) * sum_of(k + 1 + lane, wq);
         kept_it = lhs < rhs;
         close = fabs(lhs - rhs) <= kSlack * rhs && rhs > 0.0;
       }
@@ -341,8 +348,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) spec_sample_kernel(co
         double u = (double)a.u[(size_t)b * (k + 1) + n];
         if (u >= 1.0) u = 1.0 - 0x1p-24;
         if (dd < 0 || dd >= V) break;
-        const double pe = weights(n)(row(n)[dd]), qe = weights(k + 1 + n)(row(k + 1 + n)[dd]);
-        const double lhs = u * qe * row_z[n], rhs = pe * row_z[k + 1 + n];
+        const Exp64 wp = weights(n), wq = weights(k + 1 + n);
+        const double pe = wp(row(n)[dd]), qe = wq(row(k + 1 + n)[dd]);
+        const double lhs = u * qe * sum_of(n, wp), rhs = pe * sum_of(k + 1 + n, wq);
         if (fabs(lhs - rhs) <= kSlack * rhs && rhs > 0.0) {
           const double zq = exact_sum(k + 1 + n), zp = exact_sum(n);
           if (!(u * (qe / zq) < pe / zp)) break;
