@@ -253,6 +253,57 @@ def test_strided_pages(order):
     assert torch.equal(k.nan_to_num(9.0), k2.nan_to_num(9.0)) and torch.equal(v.nan_to_num(9.0), v2.nan_to_num(9.0))
 
 
+def high_keys(counts, pos, H, Hkv, Dh, page, dtype, highs, spread=0.5, seed=3):
+    """Rows whose scores are `spread` N(0, 1) but for the keys of `highs`, which
+    have score highs[j] and value 0."""
+    g = gen(seed)
+    table, pages = R.layout(counts, pos, page, seed=seed)
+    n = counts[0] + pos[0]
+    q = torch.full((counts[0], H, Dh), 0.25, dtype=dtype, device="cuda")
+    k = torch.full((pages, Hkv, page, Dh), float("nan"), dtype=dtype, device="cuda")
+    v = torch.full_like(k, float("nan"))
+    j = torch.arange(n, device="cuda")
+    kk = torch.randn((n, Hkv, Dh), generator=g, device="cuda") * (4 * spread / Dh ** 0.5)
+    vv = torch.rand((n, Hkv, Dh), generator=g, device="cuda") + 0.5
+    for at, score in highs.items():
+        kk[at] = 4.0 * score / Dh
+        vv[at] = 0.0
+    at = table[0, j // page].long(), slice(None), j % page
+    k[at], v[at] = kk.to(dtype), vv.to(dtype)
+    return q, k, v, table
+
+
+def check_high_keys(count, pos, H, Hkv, Dh, page, dtype, highs):
+    """Within the bound of the other tests, which is relative to sum p |v|: here
+    without the high keys' share. To that, for what fp16 rounds off below 2^-14:
+    a share 2^-15 of sum p |v|, and 2^-26 of the largest value (1.5)."""
+    q, k, v, table = high_keys([count], [pos], H, Hkv, Dh, page, dtype, highs)
+    out = run(q, k, v, table, [count], [pos])
+    wg.context().sync()
+    ref, bound = R.attention(q, k, v, table, [count], [pos])
+    tol = R.attention_tolerance(dtype, ref, bound, Dh, count + pos, p_eps(dtype, 0, 0, 0, 0))
+    tol = tol + 2.0 ** -15 * bound[0] + 2.0 ** -26 * 1.5
+    err = (out.double() - ref).abs()
+    assert torch.isfinite(out).all()
+    assert (err <= tol).all(), f"worst {(err / tol).max().item():.2f} of the bound"
+
+
+HIGHS = [
+    {0: 14.0}, {0: 15.0}, {0: 16.0}, {0: 17.0}, {0: 20.0}, {0: 30.0}, {0: 80.0},  # a first token far above the rest
+    {0: 17.0, 1500: 17.0}, {0: 17.0, 900: 40.0}, {700: 16.0},                     # one more later on
+    {**{j: 12.0 for j in range(0, 2500, 64)}, 0: 20.0},                           # one in every tile
+    {0: 80.0, **{j: 40.0 for j in range(64, 128)}},                               # two steps down
+    {0: 17.0, 2000: 2.0 ** 12},                                                   # and far up
+]
+
+
+@pytest.mark.parametrize("count,pos,H,Hkv,Dh,dtype", [(200, 2800, 32, 8, 128, F16), (300, 2800, 32, 8, 64, F16),
+                                                      (100, 2800, 32, 8, 256, F16), (200, 2800, 32, 8, 128, BF16)])
+@pytest.mark.parametrize("highs", HIGHS, ids=lambda h: "-".join(f"{j}:{s:g}" for j, s in sorted(h.items())[:3]))
+def test_prompt_keys_far_below_the_highest(count, pos, H, Hkv, Dh, dtype, highs):
+    check_high_keys(count, pos, H, Hkv, Dh, 64, dtype, highs)
+
+
 def test_offsets_past_32_bits():
     """Pages whose elements lie beyond 2^31 (and byte 2^32)."""
     Hkv, Dh, page = 8, 128, 64

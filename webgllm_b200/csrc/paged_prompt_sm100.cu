@@ -11,10 +11,11 @@
 //                scores, mask, maximum, exp2, P as 16-bit pairs back into the
 //                scores' tensor-memory columns (the A operand of P V), the row
 //                sum in a register; at the end O from tensor memory to `out`.
-//                The reference of the exponentials is the first tiles' maximum
-//                and follows only when a tile's P adds up to more than 2^8
-//                (so P stays well inside fp16): O is then rescaled in tensor
-//                memory, which almost never happens after the first tiles;
+//                The reference of the exponentials is the first 64 keys' maximum
+//                and moves only when the P of 64 keys add up to too much for
+//                their type or, in fp16, to so little that they would lose bits
+//                (PRange): O is then rescaled in tensor memory, which almost
+//                never happens after the first tiles;
 //   one warp     MMA: one thread issues S_t = Q_t K^T (both operands in shared
 //                memory) and O_t += P_t V (P from tensor memory, V as it lies,
 //                [key][dim], the MN-major form). The two tiles alternate:
@@ -68,6 +69,28 @@ struct PromptCfg {
   static __device__ int score_col(int t, int x) { return (t * NB + x) * KT; }
   static constexpr int kSmem = 1024 + NT * kQBytes + kStages * kStageBytes;
   static constexpr int kOCol = 256;  // tensor memory: scores at [0, 256), O after them
+};
+
+// P = 2^(s log2 e - ref) as a 16-bit number, and where the reference follows.
+// P of 64 keys are at most 64 times 2^lift where the reference is their maximum
+// (ref = maximum - lift) and may grow to a sum of `most`: no P is larger.
+// fp16 ends at 65504 and has all its bits down to 2^-14 only: a key 10 nats below
+// the reference would be rounded by more than its share, one 17 nats below be
+// lost (a first token with a high score above thousands of others), while the
+// row sum counts it in full. So P is lifted by 2^7, and 64 keys whose P add up to
+// less than `least` move the reference down to their own maximum. What is
+// rounded off below 2^-14 is then at most 64 x 2^-25 of a sum of at least 2^-4
+// (2^-15 of it), or of a sum that holds a key at the reference (2^-26). The row
+// sum, O and P carry the same factor: the quotient does not. A reference is not
+// lowered for keys whose sum is below 2^-65 of the row's: the row sum times the
+// step stays below 2^78 (and O below 2^94).
+// bf16 has the range of fp32.
+template <typename T>
+struct PRange {
+  static constexpr bool kNarrow = std::is_same<T, __half>::value;
+  static constexpr float lift = kNarrow ? 7.0f : 0.0f;
+  static constexpr float most = kNarrow ? 32768.0f : 256.0f;
+  static constexpr float least = 0x1p-4f, span = 0x1p-65f;
 };
 
 struct PromptArgs {
@@ -620,14 +643,15 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
             return v.x + v.y;
           };
           // The reference of the keys before nearly always still holds, so P is
-          // made with it and its sum tells: at most 2^8 means that no P is
-          // larger. (No maximum is taken on this path: P of 64 keys sums to 64 at
-          // most where the reference is the true maximum.)
+          // made with it and its sum tells (PRange). (No maximum is taken on this
+          // path.)
+          using R = PRange<T>;
           float sum = 0.0f;
           bool holds = false;
+          auto faint = [&]() { return R::kNarrow && sum < R::least && sum > l * R::span; };
           if (j > 0 || part > 0) {
             sum = exps();
-            holds = sum <= 256.0f;
+            holds = sum <= R::most && !faint();
             if (p < 0) {
               holds = true;  // (rows of nobody hold anything: they decide nothing for their warp)
             } else if (ref == -INFINITY) {  // nothing seen so far: still so?
@@ -641,10 +665,10 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < 64; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], sp[c], sp[c + 1]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
-            const bool grow = top > ref;
-            const float f = grow && ref > -INFINITY ? ex2(ref - top) : grow ? 0.0f : 1.0f;
-            if (grow) ref = top;
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e - R::lift;
+            const bool move = top > ref || faint();
+            const float f = move && ref > -INFINITY ? ex2(ref - top) : move ? 0.0f : 1.0f;
+            if (move) ref = top;
             l *= f;
             if (j > 0 || part > 0) {
               // O must hold all keys before these: the scores' commit says so
