@@ -304,6 +304,14 @@ def test_prompt_keys_far_below_the_highest(count, pos, H, Hkv, Dh, dtype, highs)
     check_high_keys(count, pos, H, Hkv, Dh, 64, dtype, highs)
 
 
+@pytest.mark.parametrize("count,pos,H,Hkv,Dh,dtype", [(1, 2999, 8, 2, 64, F16), (1, 2999, 8, 2, 128, F16),
+                                                      (2, 2998, 4, 2, 256, F16), (5, 2995, 32, 8, 128, F16),
+                                                      (1, 2999, 8, 2, 128, BF16)])
+@pytest.mark.parametrize("highs", HIGHS, ids=lambda h: "-".join(f"{j}:{s:g}" for j, s in sorted(h.items())[:3]))
+def test_decode_keys_far_below_the_highest(count, pos, H, Hkv, Dh, dtype, highs):
+    check_high_keys(count, pos, H, Hkv, Dh, 16, dtype, highs)
+
+
 def test_offsets_past_32_bits():
     """Pages whose elements lie beyond 2^31 (and byte 2^32)."""
     Hkv, Dh, page = 8, 128, 64

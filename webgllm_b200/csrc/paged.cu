@@ -202,8 +202,12 @@ __global__ void __launch_bounds__(64)
 //                   59 us with 16 keys, 53 with 32), and 32 query rows
 //                   take eight warps (five rows of 4 heads, 8 sequences of 4k:
 //                   52 us with four warps of both row tiles, 39 with eight).
-// P stays at fp32 precision: hi + lo 16-bit halves, two products (the tensor
-// pipe idles under the loads).
+// P is hi + lo 16-bit halves, two products (the tensor pipe idles under the
+// loads): 2^-18 of itself in bf16. In fp16 2^-22, down to 2^-2; below that what is
+// rounded off is 2^-25, so P is lifted by 2^14 against keys far below the maximum
+// (a first token with a high score above thousands of others): 2^-39 of the
+// largest. The sums carry the same factor, the quotient does not. 2^14 leaves two
+// octaves below 65504 for a reference that is rounded (scores up to 2^24).
 // A (sequence, head, rows) unit that one CTA finishes alone is written by it;
 // else each CTA leaves (max, sum, O) in the workspace and paged_join_kernel
 // adds them in order: no atomics, the same bits every time.
@@ -302,6 +306,7 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
   constexpr int kBlk = Dh / 64;                    // 64-dim blocks of a row
   constexpr int kBlkBytes = kKeys * 128;           // one block of a stage's K or V
   constexpr float kLog2e = 1.4426950408889634f;
+  constexpr float kLift = std::is_same<T, __half>::value ? 14.0f : 0.0f;  // P is 2^kLift at the maximum
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   float *red = reinterpret_cast<float *>(smem + (size_t)S * C::kStageBytes);  // [2][kRows][kRedRow]
@@ -580,7 +585,7 @@ __global__ void __launch_bounds__(SplitCfg<Dh, MT>::kThreads, SplitCfg<Dh, MT>::
             for (int nt = 1; nt < KW / 8; nt++) m = fmaxf(m, fmaxf(s[nt][2 * e], s[nt][2 * e + 1]));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float mn = fmaxf(mx[e], m * kLog2e);
+            const float mn = fmaxf(mx[e], m * kLog2e - kLift);
             f[e] = mn == -INFINITY ? 1.0f : ex2(mx[e] - mn);
             const float sub = mn == -INFINITY ? 0.0f : mn;
             mx[e] = mn;
