@@ -312,6 +312,48 @@ def test_decode_keys_far_below_the_highest(count, pos, H, Hkv, Dh, dtype, highs)
     check_high_keys(count, pos, H, Hkv, Dh, 16, dtype, highs)
 
 
+@pytest.mark.parametrize("counts,H,Hkv,Dh", [([1] * 64, 8, 2, 64), ([1] * 64, 8, 4, 128), ([1] * 32, 4, 2, 256),
+                                             ([5] * 8, 32, 8, 128), ([6] * 8, 32, 8, 64)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_decode_rows_hold_p_in_two_halves(counts, H, Hkv, Dh, dtype):
+    """Values +1 and -1 that nearly cancel, and scores that are one exact product:
+    what is left shows how P is rounded. With both halves (the second holds a
+    remainder of at most 2^-11 or 2^-8 by half its last bit) it is off by 2^-23
+    (fp16) or 2^-17 (bf16) of P, with one by 2^-11 or 2^-8: a kernel that drops a
+    half, or the prompt kernel in these rows' place, is outside the bound, as the
+    plain form with P in 16 bits is. The bound, relative to sum p |v| = 1: P; the
+    exponent s log2 e - max + 14, below 16 in size and rounded once (2^-21, by ln 2),
+    and exp2 (2^-21), both also in the row sum, and exp2 when warps are joined; fp32
+    sums over the keys, twice."""
+    B, n, pos, page = len(counts), counts[0], 15, 16
+    g = gen(B + Dh)
+    L = pos + n
+    pages = B * 2
+    table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32).view(B, 2)
+    q = torch.zeros((B * n, H, Dh), dtype=dtype, device="cuda")
+    k = torch.zeros((pages, Hkv, page, Dh), dtype=dtype, device="cuda")
+    q[..., 0] = 0.5
+    k[..., 0] = torch.randint(-128, 129, k.shape[:3], generator=g, device="cuda") / 128.0  # (8 bits: exact in bf16)
+    v = (torch.randint(0, 2, k.shape, generator=g, device="cuda") * 2 - 1).to(dtype)
+    out = run(q, k, v, table, counts, [pos] * B)
+    wg.context().sync()
+    ref, (mass, _) = R.attention(q, k, v, table, counts, [pos] * B)
+    half = torch.finfo(dtype).eps / 2
+    c = (2.0 ** -23 if dtype is F16 else 2.0 ** -17) + 2 * 2.0 ** -21 + 3 * 2.0 ** -21 + 2 * L * 2.0 ** -24
+    tol = half * (ref.abs() + c * mass) + c * mass
+    err = (out.double() - ref).abs()
+    assert (err <= tol).all(), f"worst {(err / tol).max().item():.2f} of the bound"
+    # the same with P in one number
+    i = torch.arange(L, device="cuda")
+    pg = table[:, i // page].long()
+    kk = k[pg, :, i % page, 0].double().transpose(1, 2).repeat_interleave(H // Hkv, 1)  # [B][H][L]
+    vv = v[pg, :, i % page].double().transpose(1, 2).repeat_interleave(H // Hkv, 1)
+    s = (0.5 * kk)[:, None].masked_fill((i[None] > pos + torch.arange(n, device="cuda")[:, None])[None, :, None], -1e9)
+    p = torch.exp(s - s.amax(-1, keepdim=True))
+    one = torch.einsum("bnhl,bhld->bnhd", p.to(dtype).double(), vv) / p.sum(-1, keepdim=True)
+    assert ((one.reshape(ref.shape) - ref).abs() > 2 * tol).any()
+
+
 def test_offsets_past_32_bits():
     """Pages whose elements lie beyond 2^31 (and byte 2^32)."""
     Hkv, Dh, page = 8, 128, 64

@@ -203,11 +203,12 @@ __global__ void __launch_bounds__(64)
 //                   take eight warps (five rows of 4 heads, 8 sequences of 4k:
 //                   52 us with four warps of both row tiles, 39 with eight).
 // P is hi + lo 16-bit halves, two products (the tensor pipe idles under the
-// loads): 2^-18 of itself in bf16. In fp16 2^-22, down to 2^-2; below that what is
-// rounded off is 2^-25, so P is lifted by 2^14 against keys far below the maximum
-// (a first token with a high score above thousands of others): 2^-39 of the
-// largest. The sums carry the same factor, the quotient does not. 2^14 leaves two
-// octaves below 65504 for a reference that is rounded (scores up to 2^24).
+// loads): off by up to 2^-17 of itself in bf16. In fp16 by 2^-23, down to 2^-2;
+// below that what is rounded off is 2^-25, so P is lifted by 2^14 against keys far
+// below the maximum (a first token with a high score above thousands of others):
+// 2^-39 of the largest. The sums carry the same factor, the quotient does not.
+// 2^14 leaves two octaves below 65504 for a reference that is rounded (scores up
+// to 2^24).
 // A (sequence, head, rows) unit that one CTA finishes alone is written by it;
 // else each CTA leaves (max, sum, O) in the workspace and paged_join_kernel
 // adds them in order: no atomics, the same bits every time.
