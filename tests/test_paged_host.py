@@ -90,6 +90,22 @@ def test_trim_keeps_the_window_and_the_sinks():
     assert len(c.free) == 6
 
 
+def test_trim_past_the_table_and_with_bad_sinks():
+    """A position past the table frees what it passes, and a refusal frees
+    nothing: a page is never free and in the table at once."""
+    c = cache(pages=9, batch=2)
+    c.reserve(0, 112)
+    assert c.trim(0, 1000, 16, 20) == 5  # all but the sinks' two pages
+    assert (c.table[0] >= 0).tolist() == [True, True] + [False] * 5
+    c.reserve(1, 112)
+    held = c.table[c.table >= 0].tolist()
+    assert len(set(held)) == len(held) == 9 and not c.free
+    for sinks in (-1, -20, -112):
+        with pytest.raises(wg.GpuError):
+            c.trim(1, 60, 16, sinks)
+    assert not c.free and (c.table[1] >= 0).all()
+
+
 def test_cache_refusals():
     for kw in (dict(page=24), dict(page=0), dict(pages=0), dict(batch=0), dict(max_len=0)):
         with pytest.raises(wg.ShapeError):

@@ -205,10 +205,13 @@ class PagedCache:
     def trim(self, b: int, position: int, window: int, sinks: int = 0) -> int:
         """Takes back the pages of sequence b that no row at `position` or later
         sees through the window and the sinks; returns how many."""
+        if sinks < 0:
+            raise _arg(f"sinks {sinks}")
         if window <= 0:
             return 0
         gone = 0
-        for i in range(-(-sinks // self.page_size), max(0, position - window + 1) // self.page_size):
+        past = min(max(0, position - window + 1) // self.page_size, self.max_pages)
+        for i in range(-(-sinks // self.page_size), past):
             if self.host[b][i] >= 0:
                 self.free.append(self.host[b][i])
                 self.host[b][i] = -1
