@@ -1,6 +1,8 @@
 """The paged cache and sampled speculation as a model uses them: a random-init
 decoder whose keys and values live in pages, with and without a window, and
 draft / verify / accept over it."""
+import threading
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -13,7 +15,7 @@ import decoder_reference as R  # noqa: E402
 import paged_reference as PR  # noqa: E402
 from webgllm_b200.model import DecoderConfig, DecoderModel  # noqa: E402
 from webgllm_b200.paged import PagedCache  # noqa: E402
-from webgllm_b200.speculative import SpeculativeDecoder  # noqa: E402
+from webgllm_b200.speculative import SpeculativeDecoder, spec_sample  # noqa: E402
 
 LLAMA = DecoderConfig("tiny-llama", 3, 256, 8, 2, 64, 768, 1000, 1e-5, 1e4)
 HYBRID = DecoderConfig("tiny-hybrid", 4, 256, 8, 2, 64, 512, 1000, 1e-5, 1e6, ["conv", "attn", "conv", "attn"], 3, True)
@@ -168,6 +170,54 @@ def test_low_temperature_is_greedy_speculation():
         outs.append(spec.out[:, :11].clone())
     # (a gap of logits below 1e-4 x 30 could be drawn either way: none here)
     assert torch.equal(outs[0], outs[1])
+
+
+def test_a_model_and_calls_from_another_thread():
+    """Decode steps on one thread's stream while another thread samples and
+    attends on its own: each call's launches stay on its thread's stream."""
+    m = model(LLAMA, 2, seed=3)
+    prompts = torch.randint(0, LLAMA.vocab, (2, 20), generator=gen(9), device="cuda").to(torch.int32)
+
+    def steps(n=40):
+        m.reset()
+        m.prefill(prompts)
+        logits = []
+        for _ in range(n):
+            m.decode_step()
+            logits.append(m.logits.clone())
+        return torch.stack(logits)
+
+    rows, u = torch.randn((8, 32000), generator=gen(4), device="cuda"), torch.rand((8, 1), generator=gen(5), device="cuda")
+    want, picks = steps(), spec_sample(rows, None, None, u)
+    torch.cuda.synchronize()
+    wrong, stop = [], threading.Event()
+
+    def other():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            while not stop.is_set():
+                mine = rows.clone()
+                got = spec_sample(mine, None, None, u)
+                mine.fill_(float("nan"))
+                s.synchronize()
+                if not torch.equal(got, picks):
+                    wrong.append(got)
+
+    t = threading.Thread(target=other)
+    t.start()
+    try:
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                got = steps()
+                s.synchronize()
+                assert torch.equal(got, want)
+    finally:
+        stop.set()
+        t.join()
+    assert not wrong
+    torch.cuda.synchronize()
+    m.ctx.sync()
 
 
 def test_model_refusals():

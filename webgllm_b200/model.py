@@ -313,9 +313,10 @@ class DecoderModel:
         and advances the positions."""
         if rows % self.batch or rows > self.max_rows:
             raise ValueError(f"rows {rows} for batch {self.batch} (max rows {self.max_rows})")
-        if self.fused:
-            return self._forward_fused(ids, rows)
-        return self._forward_passes(ids, rows)
+        with self.ctx.lock:  # (its launches are on one stream, whatever other threads call)
+            if self.fused:
+                return self._forward_fused(ids, rows)
+            return self._forward_passes(ids, rows)
 
     def _attend(self, lay, rows):
         self._rope_attend(lay, rows)
@@ -424,13 +425,15 @@ class DecoderModel:
             return
         cfg, L, c = self.cfg, _lib.lib(), P(self.ctx.handle)
         slots = self.conv_prefixes.shape[2]
-        for lay in self.layers:
-            if lay["type"] != "conv":
-                continue
-            s = lay["slot"]
-            self._c(L.wg_conv_restore(c, P(self.conv_prefixes[s].data_ptr()), slots, self.batch, cfg.hidden,
-                                      cfg.conv_width, P(pos_before.data_ptr()), P(self.pos.data_ptr()),
-                                      P(self.conv_state[s].data_ptr())))
+        with self.ctx.lock:
+            self.ctx.use_torch_stream()
+            for lay in self.layers:
+                if lay["type"] != "conv":
+                    continue
+                s = lay["slot"]
+                self._c(L.wg_conv_restore(c, P(self.conv_prefixes[s].data_ptr()), slots, self.batch, cfg.hidden,
+                                          cfg.conv_width, P(pos_before.data_ptr()), P(self.pos.data_ptr()),
+                                          P(self.conv_state[s].data_ptr())))
 
     def _head(self, cur, add, rows):
         """Final norm + head on each sequence's last row, greedy pick, and the

@@ -35,7 +35,15 @@ __all__ = [
 
 
 class Context:
-    """One device and one stream (the reference's Gpu, src/gpu/gl.ts:108)."""
+    """One device and one stream (the reference's Gpu, src/gpu/gl.ts:108).
+
+    Threads share a device's context: matmul, a model's forward and speculative
+    step, and the paged and sampling calls take `lock` for their stream choice and
+    the launches that go with it. Code that calls set_stream or the library itself
+    does the same if other threads use the device. The matmuls' scratch is the
+    context's too: those that may overlap on the GPU, on two streams, need
+    contexts of their own (the paged and sampling calls have their own workspaces).
+    `sync` waits for the stream that was chosen last."""
 
     def __init__(self, device: int = 0):
         self.device = device
@@ -322,10 +330,11 @@ def matmul(a, w: QuantMatrix, out=None, rows: int | None = None, out_dtype=None)
         out = torch.empty((rows, w.N), dtype=out_dtype or a.dtype, device=a.device)
     if out.shape[0] < rows or out.shape[1] != w.N or not out.is_contiguous():
         raise ShapeError(_lib.WG_INVALID_SHAPE, f"output {tuple(out.shape)} does not hold {rows} x {w.N}")
-    ctx = w.ctx
-    ctx.use_torch_stream()
-    ctx._check(_lib.lib().wg_q4_matmul(ctx.handle, ctypes.c_void_p(w.handle), ctypes.c_void_p(a.data_ptr()),
-                                       _dtype_code(a), rows, ctypes.c_void_p(out.data_ptr()), _dtype_code(out)))
+    ctx, a_type, out_type = w.ctx, _dtype_code(a), _dtype_code(out)
+    with ctx.lock:
+        ctx.use_torch_stream()
+        ctx._check(_lib.lib().wg_q4_matmul(ctx.handle, ctypes.c_void_p(w.handle), ctypes.c_void_p(a.data_ptr()),
+                                           a_type, rows, ctypes.c_void_p(out.data_ptr()), out_type))
     return out
 
 

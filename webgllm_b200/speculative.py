@@ -34,8 +34,6 @@ from . import _lib
 from .model import DecoderConfig, DecoderModel
 from .q4 import context, host_calls
 
-P = ctypes.c_void_p
-
 
 def draft_config(target: DecoderConfig) -> DecoderConfig:
     """Config 2's layout with the target's vocabulary."""
@@ -177,11 +175,9 @@ class SpeculativeDecoder:
         if self.temperature:
             spec_sample(self.t_logits, self.d_logits if k else None, self.drafts if k else None, self.u,
                         temperature=self.temperature, out=self.picks)
-        L = _lib.lib()
-        t._c(L.wg_spec_accept(P(t.ctx.handle), P(self.drafts.data_ptr()), P(self.picks.data_ptr()), t.batch, k,
-                              P(t.pos.data_ptr()), P(d.pos.data_ptr()), P(t.next_id.data_ptr()),
-                              P(d.next_id.data_ptr()), P(self.out.data_ptr()), self.out.shape[1],
-                              P(self.out_len.data_ptr()), P(self.accepted.data_ptr())))
+        t.ctx.enqueue(_lib.lib().wg_spec_accept, self.drafts.data_ptr(), self.picks.data_ptr(), t.batch, k,
+                      t.pos.data_ptr(), d.pos.data_ptr(), t.next_id.data_ptr(), d.next_id.data_ptr(),
+                      self.out.data_ptr(), self.out.shape[1], self.out_len.data_ptr(), self.accepted.data_ptr())
         t.restore_prefix(self.pos_t0)
         d.restore_prefix(self.pos_d0)
 
