@@ -89,3 +89,18 @@ def test_speculative_accept_holds_the_stream(recorded):
     s.out_len = s.accepted = s.pos_t0 = s.pos_d0 = torch.zeros(1, dtype=torch.int32)
     s.step()
     held(calls, "wg_set_stream", "wg_spec_accept")
+
+
+def test_a_refusal_is_read_before_another_call(recorded, monkeypatch):
+    """The context's last error belongs to the call that failed."""
+    ctx, _ = recorded
+    seen = []
+
+    def check(status, handle=None):
+        seen.append((status, ctx.lock.locked()))
+        raise _lib.GpuError(status, "refused")
+
+    monkeypatch.setattr(q4, "check", check)
+    with pytest.raises(_lib.GpuError):
+        ctx.enqueue(lambda handle: 7)
+    assert seen == [(7, True)] and not ctx.lock.locked()

@@ -117,7 +117,8 @@ def workspace_bytes(device: int, head_dim: int) -> int:
     if n is None:
         b = ctypes.c_size_t()
         ctx = context(device)
-        ctx._check(_lib.lib().wg_paged_attention_workspace(ctx.handle, head_dim, ctypes.byref(b)))
+        with ctx.lock:
+            ctx._check(_lib.lib().wg_paged_attention_workspace(ctx.handle, head_dim, ctypes.byref(b)))
         n = _workspace_bytes[device, head_dim] = b.value
     return n
 

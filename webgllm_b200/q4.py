@@ -58,13 +58,15 @@ class Context:
         as it was."""
         here = _current_device()
         stream = _raw_stream(self.device)
-        with self.lock:
-            _lib.lib().wg_set_stream(self.handle, stream if stream else _CUDA_STREAM_LEGACY)
-            status = fn(self.handle, *args)
-        if here != self.device:
-            _set_device(here)
-        if status:
-            self._check(status)
+        try:
+            with self.lock:
+                _lib.lib().wg_set_stream(self.handle, stream if stream else _CUDA_STREAM_LEGACY)
+                status = fn(self.handle, *args)
+                if status:
+                    self._check(status)  # (the error's text is this call's only as long as the lock is held)
+        finally:
+            if here != self.device:
+                _set_device(here)
 
     def close(self) -> None:
         if self.handle:

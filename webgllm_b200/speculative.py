@@ -76,7 +76,8 @@ def spec_sample(target: torch.Tensor, draft: torch.Tensor | None, drafts: torch.
             raise _lib.GpuError(_lib.WG_INVALID_ARGUMENT, f"{what} must be contiguous {dt} on CUDA device {device}")
     ctx, L = context(device), _lib.lib()
     need = ctypes.c_size_t()
-    ctx._check(L.wg_spec_sample_workspace(ctx.handle, batch, k, V, ctypes.byref(need)))
+    with ctx.lock:
+        ctx._check(L.wg_spec_sample_workspace(ctx.handle, batch, k, V, ctypes.byref(need)))
     # from torch's allocator: safe on any stream and inside a graph
     ws = torch.empty(max(need.value, 8), dtype=torch.uint8, device=target.device)
     ctx.enqueue(L.wg_spec_sample, target.data_ptr(), draft.data_ptr() if k else None, drafts.data_ptr() if k else None,
