@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import WG_BF16, WG_F16, GpuError, ShapeError, wg_paged_kv
-from .q4 import context, host_calls
+from .q4 import context_of, host_calls
 
 __all__ = ["PagedCache", "attention_paged", "rope_kv_paged"]
 
@@ -106,8 +106,8 @@ def rope_kv_paged(qkv: torch.Tensor, pos: torch.Tensor, k: torch.Tensor, v: torc
         _check_out(out, k.dtype, (rows, heads, dim), device)
     p = _int32(pos, "pos", (batch,), device)
     rs = None if row_start is None else _int32(row_start, "row_start", (batch + 1,), device)
-    context(device).enqueue(_lib.lib().wg_paged_rope_kv, qkv.data_ptr(), rows, batch, rs, heads, hkv, dim, p, theta,
-                            _ptr(q_norm), _ptr(k_norm), eps, out.data_ptr(), ctypes.byref(kv))
+    context_of(device).enqueue(_lib.lib().wg_paged_rope_kv, qkv.data_ptr(), rows, batch, rs, heads, hkv, dim, p, theta,
+                               _ptr(q_norm), _ptr(k_norm), eps, out.data_ptr(), ctypes.byref(kv))
     return out
 
 
@@ -116,7 +116,7 @@ def workspace_bytes(device: int, head_dim: int) -> int:
     n = _workspace_bytes.get((device, head_dim))
     if n is None:
         b = ctypes.c_size_t()
-        ctx = context(device)
+        ctx = context_of(device)
         with ctx.lock:
             ctx._check(_lib.lib().wg_paged_attention_workspace(ctx.handle, head_dim, ctypes.byref(b)))
         n = _workspace_bytes[device, head_dim] = b.value
@@ -157,8 +157,8 @@ def attention_paged(q: torch.Tensor, pos: torch.Tensor, k: torch.Tensor, v: torc
         workspace = torch.empty(workspace_bytes(device, dim), dtype=torch.uint8, device=k.device)
     elif workspace.get_device() != device or not workspace.is_contiguous():
         raise _arg(f"workspace must be contiguous on CUDA device {device}")
-    context(device).enqueue(_lib.lib().wg_paged_attention, q.data_ptr(), rows, batch, rs, heads, hkv, dim, p,
-                            ctypes.byref(kv), window, sinks, out.data_ptr(), workspace.data_ptr(), workspace.nbytes)
+    context_of(device).enqueue(_lib.lib().wg_paged_attention, q.data_ptr(), rows, batch, rs, heads, hkv, dim, p,
+                               ctypes.byref(kv), window, sinks, out.data_ptr(), workspace.data_ptr(), workspace.nbytes)
     return out
 
 

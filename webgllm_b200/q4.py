@@ -173,6 +173,20 @@ def context(device: int | None = None) -> Context:
         return ctx
 
 
+def context_of(device: int) -> Context:
+    """context(device) for calls on tensors of that device: a new context makes
+    its device the current one, and the caller's stays as it was."""
+    ctx = _contexts.get(device)
+    if ctx is None:
+        here = _current_device()
+        try:
+            ctx = context(device)
+        finally:
+            if here != device:
+                _set_device(here)
+    return ctx
+
+
 @functools.cache
 def host_calls():
     """webgllm_b200._host (csrc/host/calls.cpp: the checks and the call of the

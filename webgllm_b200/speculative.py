@@ -32,7 +32,7 @@ import torch
 
 from . import _lib
 from .model import DecoderConfig, DecoderModel
-from .q4 import context, host_calls
+from .q4 import context_of, host_calls
 
 
 def draft_config(target: DecoderConfig) -> DecoderConfig:
@@ -74,7 +74,7 @@ def spec_sample(target: torch.Tensor, draft: torch.Tensor | None, drafts: torch.
             raise _lib.ShapeError(_lib.WG_INVALID_SHAPE, f"{what} {tuple(t.shape)} must be {shape}")
         if t.dtype is not dt or t.get_device() != device or not t.is_contiguous():
             raise _lib.GpuError(_lib.WG_INVALID_ARGUMENT, f"{what} must be contiguous {dt} on CUDA device {device}")
-    ctx, L = context(device), _lib.lib()
+    ctx, L = context_of(device), _lib.lib()
     need = ctypes.c_size_t()
     with ctx.lock:
         ctx._check(L.wg_spec_sample_workspace(ctx.handle, batch, k, V, ctypes.byref(need)))
