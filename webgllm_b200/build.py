@@ -46,27 +46,33 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 
 def build_host(verbose: bool = False) -> Path | None:
     """Compile csrc/host/ into the Python module _host.so against the installed
-    torch. None (and a line on stderr) where there is no torch to build with:
-    the calls then go through Python's code."""
+    torch. None (and a line on stderr, and no module) where that cannot be done -
+    no torch, one without CUDA, no headers, no compiler: the calls then go
+    through Python's code."""
     srcs = sorted((CSRC / "host").glob("*.cpp"))
     stamp = OBJ_DIR / "host_torch"
     try:
         import torch
         from torch.utils.cpp_extension import CUDA_HOME, include_paths, library_paths
-    except ImportError as e:
+
+        built_for = stamp.read_text() if stamp.exists() else ""
+        if built_for == torch.__version__ and not _stale(HOST, [*srcs, *(ROOT / "include").glob("*.h")]):
+            return HOST
+        includes = [*include_paths(), sysconfig.get_paths()["include"],
+                    str(Path(CUDA_HOME or "/usr/local/cuda") / "include")]
+        made = OBJ_DIR / HOST.name
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes),
+               *map(str, srcs), "-o", str(made), *(f for p in library_paths() for f in (f"-L{p}", f"-Wl,-rpath,{p}")),
+               "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        subprocess.run(cmd, check=True)
+        made.replace(HOST)
+    except (ImportError, OSError, subprocess.CalledProcessError) as e:
+        HOST.unlink(missing_ok=True)  # (one of another build or torch)
         print(f"{HOST.name} not built: {e}", file=sys.stderr)
         return None
-    built_for = stamp.read_text() if stamp.exists() else ""
-    if built_for == torch.__version__ and not _stale(HOST, [*srcs, *(ROOT / "include").glob("*.h")]):
-        return HOST
-    includes = [*include_paths(), sysconfig.get_paths()["include"], str(Path(CUDA_HOME or "/usr/local/cuda") / "include")]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes),
-           *map(str, srcs), "-o", str(HOST), *(f for p in library_paths() for f in (f"-L{p}", f"-Wl,-rpath,{p}")),
-           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
     stamp.write_text(torch.__version__)
     return HOST
 
