@@ -1,4 +1,6 @@
 """The module of native calls: what build and import do where it cannot be had."""
+import sys
+
 import pytest
 
 pytest.importorskip("torch")
@@ -30,3 +32,34 @@ def test_headers_that_are_missing(target, monkeypatch, capfd):
     monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {"include": "/nonexistent"})
     assert build.build_host() is None
     assert not build.HOST.exists() and "not built" in capfd.readouterr().err
+
+
+def test_a_module_of_another_torch_is_not_used(monkeypatch):
+    """After an upgrade without a rebuild the module would read the new torch's
+    tensors by the old one's layout: it is left alone, before any call."""
+    from types import SimpleNamespace
+
+    import webgllm_b200
+    from webgllm_b200 import q4
+
+    def used(*args):
+        raise AssertionError("bound")
+
+    for built_for in ("2.0.0 3.12", "", build.host_target().replace(" ", "x ")):
+        old = SimpleNamespace(built_for=built_for, bind=used)
+        monkeypatch.setitem(sys.modules, "webgllm_b200._host", old)
+        monkeypatch.setattr(webgllm_b200, "_host", old, raising=False)
+        assert q4.host_calls.__wrapped__() is None
+    old = SimpleNamespace(bind=used)  # from before modules said so
+    monkeypatch.setitem(sys.modules, "webgllm_b200._host", old)
+    monkeypatch.setattr(webgllm_b200, "_host", old, raising=False)
+    assert q4.host_calls.__wrapped__() is None
+
+
+def test_the_module_says_what_it_is_built_for():
+    from webgllm_b200 import q4
+
+    host = q4.host_calls()
+    if host is None:
+        pytest.skip("webgllm_b200._host is not built")
+    assert host.built_for == build.host_target()

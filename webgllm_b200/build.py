@@ -44,6 +44,13 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def host_target() -> str:
+    """What _host.so is compiled against: it is used with nothing else."""
+    import torch
+
+    return f"{torch.__version__} {sys.version_info[0]}.{sys.version_info[1]}"
+
+
 def build_host(verbose: bool = False) -> Path | None:
     """Compile csrc/host/ into the Python module _host.so against the installed
     torch. None (and a line on stderr, and no module) where that cannot be done -
@@ -55,15 +62,16 @@ def build_host(verbose: bool = False) -> Path | None:
         import torch
         from torch.utils.cpp_extension import CUDA_HOME, include_paths, library_paths
 
+        target = host_target()
         built_for = stamp.read_text() if stamp.exists() else ""
-        if built_for == torch.__version__ and not _stale(HOST, [*srcs, *(ROOT / "include").glob("*.h")]):
+        if built_for == target and not _stale(HOST, [*srcs, *(ROOT / "include").glob("*.h")]):
             return HOST
         includes = [*include_paths(), sysconfig.get_paths()["include"],
                     str(Path(CUDA_HOME or "/usr/local/cuda") / "include")]
         made = OBJ_DIR / HOST.name
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes),
-               *map(str, srcs), "-o", str(made), *(f for p in library_paths() for f in (f"-L{p}", f"-Wl,-rpath,{p}")),
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DWG_HOST_TARGET="{target}"',
+               *(f"-I{i}" for i in includes), *map(str, srcs), "-o", str(made), *(f for p in library_paths() for f in (f"-L{p}", f"-Wl,-rpath,{p}")),
                "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
@@ -73,7 +81,7 @@ def build_host(verbose: bool = False) -> Path | None:
         HOST.unlink(missing_ok=True)  # (one of another build or torch)
         print(f"{HOST.name} not built: {e}", file=sys.stderr)
         return None
-    stamp.write_text(torch.__version__)
+    stamp.write_text(target)
     return HOST
 
 

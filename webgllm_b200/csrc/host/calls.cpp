@@ -299,5 +299,8 @@ PyMODINIT_FUNC PyInit__host() {
   s_acquire_ = PyUnicode_InternFromString("acquire");
   s_release_ = PyUnicode_InternFromString("release");
   if (!s_handle_ || !s_lock_ || !s_acquire_ || !s_release_) return nullptr;
-  return PyModule_Create(&module);
+  PyObject *m = PyModule_Create(&module);
+  // read before bind() by whoever imports this: another torch lays tensors out otherwise
+  if (m && PyModule_AddStringConstant(m, "built_for", WG_HOST_TARGET) < 0) Py_CLEAR(m);
+  return m;
 }

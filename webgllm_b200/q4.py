@@ -191,14 +191,18 @@ def context_of(device: int) -> Context:
 def host_calls():
     """webgllm_b200._host (csrc/host/calls.cpp: the checks and the call of the
     serving operators as one native step) bound to the library, or None where
-    it is not built for this torch: the Python code then does the same, slower."""
+    it is not built for this torch and Python: the Python code then does the
+    same, slower."""
     try:
         import torch  # noqa: F401  (its libraries)
 
         from . import _host
+        from .build import host_target
 
         L = _lib.lib()
     except ImportError:
+        return None
+    if getattr(_host, "built_for", None) != host_target():
         return None
     _host.bind(_contexts, *(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
         L.wg_set_stream, L.wg_paged_rope_kv, L.wg_paged_attention, L.wg_paged_attention_workspace, L.wg_spec_sample,
