@@ -51,7 +51,8 @@ typedef struct wg_paged_kv {
  * an optional RMS norm over Dh (q_norm / k_norm fp32 [Dh], NULL: none), then
  * rotate-half RoPE of the pairs (j, j + Dh/2) by p theta^(-2j/Dh) (the angle
  * reduced in 64 bits: exact to fp32 at any position). q_out [rows][H][Dh]
- * in the cache's dtype, scaled by 1/sqrt(Dh); k (rotated) and v go to the row's page.
+ * in the cache's dtype, scaled by 1/sqrt(Dh), not overlapping qkv; k (rotated) and v
+ * go to the row's page.
  * Dh in {64, 128, 256}. A row past the table, or whose page entry names no
  * page, is not appended and reported by wg_sync. */
 int wg_paged_rope_kv(wg_ctx *ctx, const float *qkv, int rows, int batch, const int32_t *row_start, int H, int Hkv,
@@ -71,7 +72,7 @@ int wg_paged_rope_kv(wg_ctx *ctx, const float *qkv, int rows, int batch, const i
  * `workspace` (16-byte aligned device memory of at least
  * wg_paged_attention_workspace bytes, any content) holds the partial sums of
  * sequences that several CTAs share: calls that may overlap on the GPU need
- * one each. */
+ * one each, which overlaps neither q nor out. */
 int wg_paged_attention(wg_ctx *ctx, const void *q, int rows, int batch, const int32_t *row_start, int H, int Hkv,
                        int Dh, const int32_t *pos, const wg_paged_kv *kv, int window, int sinks, void *out,
                        void *workspace, size_t workspace_bytes);

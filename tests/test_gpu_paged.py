@@ -562,6 +562,37 @@ def test_c_level_refusals():
     assert "wg_paged_rope_kv" in L.wg_last_error(c.handle).decode()
 
 
+def test_overlapping_tensors_are_refused():
+    """What a call writes shares no memory with what it reads in another order
+    (nothing is launched)."""
+    L, c = _lib.lib(), wg.context()
+    c.use_torch_stream()
+    t = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+    d = t.data_ptr()
+    n = ctypes.c_size_t()
+    assert L.wg_paged_attention_workspace(c.handle, 64, ctypes.byref(n)) == 0
+    pages = torch.zeros((2, 2, 2, 16, 64), dtype=F16, device="cuda")
+    table = torch.tensor([[0, -1], [1, -1]], dtype=torch.int32, device="cuda")
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    kv = _lib.wg_paged_kv(pages[0].data_ptr(), pages[1].data_ptr(), table.data_ptr(), _lib.WG_F16, 2, 16, 2, 0, 0, 0)
+    A, qkv, q = _lib.WG_INVALID_ARGUMENT, 2 * 8 * 64 * 4, 2 * 4 * 64 * 2  # bytes of 2 rows of 4 + 2 x 2 heads
+
+    def append(out):
+        return L.wg_paged_rope_kv(c.handle, d + q, 2, 2, None, 4, 2, 64, pos.data_ptr(), 1e4, None, None, 1e-5, d + out,
+                                  ctypes.byref(kv))
+
+    def attend(ws):
+        return L.wg_paged_attention(c.handle, d + 4096, 2, 2, None, 4, 2, 64, pos.data_ptr(), ctypes.byref(kv), 0, 0,
+                                    d + 4096 + q, d + ws, n.value)
+
+    for out in (16, q, q + qkv - 16):
+        assert append(out) == A and "overlap" in L.wg_last_error(c.handle).decode()
+    for ws in (16, 4096, 4096 + q, 4096 + 2 * q - 16):
+        assert attend(ws) == A and "overlap" in L.wg_last_error(c.handle).decode()
+    assert append(0) == 0 and append(q + qkv) == 0 and attend(4096 + 2 * q) == 0
+    c.sync()
+
+
 def test_another_current_stream_is_honoured():
     """Inputs made on a side stream are used in its order."""
     H, Hkv, Dh, page = 8, 2, 64, 16

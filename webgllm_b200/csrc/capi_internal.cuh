@@ -67,6 +67,12 @@ struct wg_q4mat {
 
 
 namespace wg {
+// Whether two buffers share memory (one without a pointer or bytes shares none).
+inline bool overlap(const void *a, size_t na, const void *b, size_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x && y && na && nb && (x < y ? y - x < na : x - y < nb);
+}
+
 struct GemvArgs;
 // Whether a GEMV launch of these arguments goes to the wide kernel (capi.cu).
 bool gemv_use_wide(const wg_ctx *ctx, const GemvArgs &a);

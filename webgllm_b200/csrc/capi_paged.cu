@@ -83,6 +83,9 @@ int wg_paged_rope_kv(wg_ctx *ctx, const float *qkv, int rows, int batch, const i
   if (!aligned(qkv, 16) || !aligned(q_out, 16) || !aligned(pos, 4) || !aligned(row_start, 4) || !aligned(q_norm, 4) ||
       !aligned(k_norm, 4))
     return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_rope_kv: misaligned tensor");
+  const size_t elems = (size_t)rows * H * Dh;
+  if (wg::overlap(qkv, (size_t)rows * (H + 2 * (size_t)Hkv) * Dh * 4, q_out, elems * 2))
+    return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_rope_kv: qkv and q_out overlap");
   return finish(ctx,
                 wg::launch_paged_rope_kv(qkv, wg::PagedRows{row_start, pos, rows, batch}, H, Hkv, Dh, theta, q_norm,
                                          k_norm, eps, q_out, *kv, ctx->d_flags, ctx->num_sms, ctx->stream, ctx->pdl),
@@ -106,13 +109,15 @@ int wg_paged_attention(wg_ctx *ctx, const void *q, int rows, int batch, const in
   if (!q || !pos || !out || !workspace) return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_attention: null");
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(pos, 4) || !aligned(row_start, 4))
     return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_attention: misaligned tensor");
-  const long long bytes = (long long)rows * H * Dh * 2;
-  if ((const char *)q < (const char *)out + bytes && (const char *)out < (const char *)q + bytes)
+  const size_t bytes = (size_t)rows * H * Dh * 2;
+  if (wg::overlap(q, bytes, out, bytes))
     return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_attention: q and out overlap");
   const size_t need = wg::paged_attention_workspace(Dh, ctx->num_sms);
   if (workspace_bytes < need)
     return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_attention: a workspace of %zu bytes, %zu needed", workspace_bytes,
                  need);
+  if (wg::overlap(workspace, need, q, bytes) || wg::overlap(workspace, need, out, bytes))
+    return pfail(ctx, WG_INVALID_ARGUMENT, "wg_paged_attention: the workspace overlaps q or out");
   return finish(ctx,
                 wg::launch_paged_attention(q, wg::PagedRows{row_start, pos, rows, batch}, H, Hkv, Dh, *kv, window,
                                            sinks, out, workspace, ctx->d_flags, ctx->num_sms, ctx->stream, ctx->pdl),
