@@ -163,7 +163,7 @@ int wg_spec_accept(wg_ctx *ctx, const int32_t *drafts, const int32_t *picks, int
  * by wg_sync. k <= 32, V <= 2^21, (2k + 1) batch <= 65535, temperature in
  * [1e-4, 1e4]. `workspace` (8-byte aligned device memory of at least
  * wg_spec_sample_workspace bytes, any content): calls that may overlap on the
- * GPU need one each. */
+ * GPU need one each. picks and workspace overlap no other tensor. */
 int wg_spec_sample(wg_ctx *ctx, const float *target, const float *draft, const int32_t *drafts, int batch, int k,
                    int V, double temperature, const float *u, int32_t *picks, void *workspace,
                    size_t workspace_bytes);

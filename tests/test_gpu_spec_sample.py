@@ -340,3 +340,29 @@ def test_refusals():
         assert call(**kw) == st, kw
     assert L.wg_spec_sample_workspace(c.handle, 1, 1, 8, ctypes.byref(n)) == 0 and n.value == 24
     assert L.wg_spec_sample_workspace(c.handle, 1, 40, 8, ctypes.byref(n)) == I
+
+
+def test_overlapping_tensors_are_refused():
+    """picks and the workspace share no memory with the inputs or each other
+    (nothing is launched)."""
+    c, L = wg.context(), _lib.lib()
+    c.use_torch_stream()
+    B, k, V = 2, 1, 8
+    x = torch.zeros(4096, device="cuda").data_ptr()
+    at = dict(target=x, draft=x + 128, drafts=x + 192, u=x + 256, picks=x + 512, ws=x + 1024)
+    size = dict(target=128, draft=64, drafts=8, u=16, picks=16, ws=48)
+
+    def call(**kw):
+        a = {**at, **kw}
+        return L.wg_spec_sample(c.handle, a["target"], a["draft"], a["drafts"], B, k, V, 1.0, a["u"], a["picks"], a["ws"],
+                                1024)
+
+    A = _lib.WG_INVALID_ARGUMENT
+    for what in ("target", "draft", "drafts", "u", "ws"):
+        for p in (at[what], at[what] + size[what] - 4, at[what] - 12):
+            assert call(picks=p) == A and "overlap" in L.wg_last_error(c.handle).decode(), what
+    for what in ("target", "draft", "drafts", "u", "picks"):
+        for p in (at[what], at[what] + size[what] - 8, at[what] - 40):
+            assert call(ws=p) == A and "overlap" in L.wg_last_error(c.handle).decode(), what
+    assert call() == 0 and call(picks=x + 272) == 0
+    c.sync()

@@ -281,6 +281,14 @@ int wg_spec_sample(wg_ctx *ctx, const float *target, const float *draft, const i
   if (((uintptr_t)workspace & 7u) || workspace_bytes < need)
     return dfail(ctx, WG_INVALID_ARGUMENT, "wg_spec_sample: a workspace of %zu bytes, %zu needed (8-byte aligned)",
                  workspace_bytes, need);
+  const size_t tokens = (size_t)batch * (k + 1) * 4, row = (size_t)batch * V * 4;
+  const struct {
+    const void *p;
+    size_t bytes;
+  } in[] = {{target, row * (k + 1)}, {draft, row * k}, {drafts, (size_t)batch * k * 4}, {u, tokens}};
+  bool shared = wg::overlap(picks, tokens, workspace, need);
+  for (const auto &t : in) shared |= wg::overlap(picks, tokens, t.p, t.bytes) || wg::overlap(workspace, need, t.p, t.bytes);
+  if (shared) return dfail(ctx, WG_INVALID_ARGUMENT, "wg_spec_sample: picks or the workspace overlap another tensor");
   return finish(ctx,
                 wg::launch_spec_sample(target, draft, drafts, batch, k, V, temperature, u, picks, workspace,
                                        ctx->d_flags, ctx->num_sms, ctx->stream, ctx->pdl),
