@@ -354,6 +354,26 @@ def test_decode_rows_hold_p_in_two_halves(counts, H, Hkv, Dh, dtype):
     assert ((one.reshape(ref.shape) - ref).abs() > 2 * tol).any()
 
 
+@pytest.mark.parametrize("count,H,Hkv", [(1, 8, 2), (5, 32, 8), (200, 32, 8)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("score", [2.0 ** 15, 2.0 ** 22, -2.0 ** 23, 2.0 ** 23])
+def test_scores_of_any_size(count, H, Hkv, dtype, score):
+    """Half of the keys share one exact score far above the others': the result
+    is their values' mean, however the reference of the exponentials is rounded.
+    Off by P's rounding (the same for all), the sums' and the output's."""
+    Dh, page, pos = 128, 16, 700
+    q, k, v, table = make([count], [pos], H, Hkv, Dh, page, dtype, seed=count)
+    q.fill_(16.0)
+    top = torch.rand(k.shape[:3], generator=gen(5), device="cuda") < 0.5
+    high, low = max(score, 0.0), min(score, 0.0)
+    k.copy_(torch.where(top, high, low)[..., None] / (16 * Dh))
+    out = run(q, k, v, table, [count], [pos])
+    wg.context().sync()
+    ref, (mass, _) = R.attention(q, k, v, table, [count], [pos])
+    c = p_eps(dtype, 0, 0, 0, 0) + 2 * 2.0 ** -21 + 2 * (pos + count) * 2.0 ** -24
+    assert ((out.double() - ref).abs() <= torch.finfo(dtype).eps / 2 * (ref.abs() + c * mass) + c * mass).all()
+
+
 def test_offsets_past_32_bits():
     """Pages whose elements lie beyond 2^31 (and byte 2^32)."""
     Hkv, Dh, page = 8, 128, 64
