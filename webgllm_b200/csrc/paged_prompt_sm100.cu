@@ -82,15 +82,18 @@ struct PromptCfg {
 // rounded off below 2^-14 is then at most 64 x 2^-25 of a sum of at least 2^-4
 // (2^-15 of it), or of a sum that holds a key at the reference (2^-26). The row
 // sum, O and P carry the same factor: the quotient does not. A reference is not
-// lowered for keys whose sum is below 2^-65 of the row's: the row sum times the
-// step stays below 2^78 (and O below 2^94).
+// lowered where the row sum would pass 2^80 (and O 2^96): such keys are below
+// 2^-60 of it. The test stands behind those for rows of nobody and for rows that
+// have seen nothing: in front of them it costs 16 bytes of spills and 2 % (8192
+// rows as calls: 517 us, so 509, without any 504).
 // bf16 has the range of fp32.
 template <typename T>
 struct PRange {
   static constexpr bool kNarrow = std::is_same<T, __half>::value;
   static constexpr float lift = kNarrow ? 7.0f : 0.0f;
   static constexpr float most = kNarrow ? 32768.0f : 256.0f;
-  static constexpr float least = 0x1p-4f, span = 0x1p-65f;
+  static constexpr float least = 0x1p-4f, span = 0x1p80f;
+  static constexpr float drop = 11.0f;  // lift - log2(least): the maximum of 64 keys that add up to less is as far below
 };
 
 struct PromptArgs {
@@ -648,10 +651,8 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
           using R = PRange<T>;
           float sum = 0.0f;
           bool holds = false;
-          auto faint = [&]() { return R::kNarrow && sum < R::least && sum > l * R::span; };
           if (j > 0 || part > 0) {
             sum = exps();
-            holds = sum <= R::most && !faint();
             if (p < 0) {
               holds = true;  // (rows of nobody hold anything: they decide nothing for their warp)
             } else if (ref == -INFINITY) {  // nothing seen so far: still so?
@@ -659,6 +660,8 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
 #pragma unroll
               for (int c = 0; c < 64; c += 2) top = max3(top, sp[c], sp[c + 1]);
               holds = !(top > -INFINITY) && !isnan(sum);
+            } else {
+              holds = sum <= R::most && !(R::kNarrow && sum < R::least && sum > 0.0f);
             }
           }
           if (!__all_sync(0xffffffffu, holds)) {
@@ -666,8 +669,9 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 64; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], sp[c], sp[c + 1]);
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e - R::lift;
-            const bool move = top > ref || faint();
-            const float f = move && ref > -INFINITY ? ex2(ref - top) : move ? 0.0f : 1.0f;
+            float f = ref > -INFINITY ? ex2(ref - top) : 0.0f;
+            const bool move = top > ref || (R::kNarrow && top < ref - R::drop && l * f < R::span);
+            if (!move) f = 1.0f;
             if (move) ref = top;
             l *= f;
             if (j > 0 || part > 0) {
@@ -794,7 +798,11 @@ cudaError_t prompt_t(const void *q, PromptArgs A, const wg_paged_kv &kv, int num
 }  // namespace
 
 // Which of the two kernels, from the rows a sequence has on average (lengths are
-// on the device, and both kernels' times are proportional to them). This one
+// on the device). For sequences of about as many rows both times are proportional
+// to the keys; in a call of a chunk and single rows they are not, since only the
+// split kernel spreads one row's keys over the machine (H 32, Hkv 8, Dh 128: 512
+// rows and a row of 131k keys 1709 us, in two calls 17 and 93; 2048 rows and 63
+// single ones of up to 16k keys 817, in two calls 51 and 404). This one
 // takes rounds of num_sms units of 256 rows (128 at Dh = 256), a CTA for all keys
 // of a unit; the split kernel spreads row tiles of 32 (16 at Dh = 256) over the
 // machine. Per 64 keys, a round here costs what kSplitWorth row tiles an SM cost
