@@ -16,8 +16,8 @@
  * Rows. `rows` rows belong to `batch` sequences, in order: rows / batch each
  * (row_start NULL), or sequence b's rows are row_start[b] ..
  * row_start[b + 1] - 1 (int32 [batch + 1] on the device, ascending; rows
- * outside [row_start[0], row_start[batch]) belong to nobody: they are not
- * read and their outputs stay as they were). pos int32 [batch] (device) is
+ * outside [row_start[0], row_start[batch]) belong to nobody: what they hold
+ * changes nothing and their outputs stay as they were). pos int32 [batch] (device) is
  * the position of each sequence's first row. A row at a negative position is
  * padding: it appends nothing, sees nothing and its outputs are zeros.
  */
@@ -64,11 +64,14 @@ int wg_paged_rope_kv(wg_ctx *ctx, const float *qkv, int rows, int batch, const i
  * window > 0 only those with j > p - window or j < sinks (a sliding window
  * and the first `sinks` positions, which stay visible). out = softmax(q . k)
  * v, a row that sees nothing gets zeros. q (scaled) and out [rows][H][Dh] in
- * the cache's dtype, not overlapping. Dh in {64, 128, 256}, H a multiple of Hkv, any rows per sequence
- * (one for a decode step, k + 1 to verify drafts, a prompt's chunk). What a
- * row does not see may hold anything, NaN included. A visible position whose
- * page entry names no page is left out and reported by wg_sync; positions
- * past the table are left out.
+ * the cache's dtype, not overlapping. Dh in {64, 128, 256}, H a multiple of
+ * Hkv, any rows per sequence (one for a decode step, k + 1 to verify drafts, a
+ * prompt's chunk). One kernel serves a call, chosen by its sequences' rows on
+ * average: prompt chunks and single rows over long contexts are faster in two
+ * calls. Scores (q . k) are below 2^24 in size. What a row does not see may
+ * hold anything, NaN included. A visible position whose page entry names no
+ * page is left out and reported by wg_sync; positions past the table are left
+ * out.
  * `workspace` (16-byte aligned device memory of at least
  * wg_paged_attention_workspace bytes, any content) holds the partial sums of
  * sequences that several CTAs share: calls that may overlap on the GPU need

@@ -71,7 +71,8 @@ def build_host(verbose: bool = False) -> Path | None:
         made = OBJ_DIR / HOST.name
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DWG_HOST_TARGET="{target}"',
-               *(f"-I{i}" for i in includes), *map(str, srcs), "-o", str(made), *(f for p in library_paths() for f in (f"-L{p}", f"-Wl,-rpath,{p}")),
+               *(f"-I{i}" for i in includes), *map(str, srcs), "-o", str(made),
+               *(f for p in library_paths() for f in (f"-L{p}", f"-Wl,-rpath,{p}")),
                "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
