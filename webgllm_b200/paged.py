@@ -131,7 +131,8 @@ def attention_paged(q: torch.Tensor, pos: torch.Tensor, k: torch.Tensor, v: torc
     row sees the keys up to its own position; else the last `window` of them
     and the first `sinks` positions. `workspace`: a uint8 tensor of
     workspace_bytes(...) that no overlapping call uses (default: a new one from
-    torch's allocator, safe on any stream and inside a graph)."""
+    torch's allocator, safe on any stream and inside a graph). Prompt chunks and
+    single rows over long contexts are faster in two calls than in one."""
     host = host_calls()
     if host is not None:
         done = host.attention_paged(q, pos, k, v, table, window, sinks, row_start, out, workspace)
